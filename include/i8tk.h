@@ -401,6 +401,84 @@ int i8tk_transpose_int8_weights(const int8_t* W1, const int8_t* W2,
                                 int8_t* W1T, int8_t* W2T,
                                 int d_model, int d_ff, i8tk_stream_t stream);
 
+/* ------------------------------------------------------------------------
+ * Grouped-head layers: heads query heads share kv_heads key/value heads (query head h reads key
+ * head h / (heads / kv_heads)).  The reference has one key head per query head throughout; these
+ * entries have no counterpart among its launchers.  16-bit inputs are fp16 or bf16.
+ * ---------------------------------------------------------------------- */
+enum i8tk_dtype { I8TK_F16 = 0, I8TK_BF16 = 1 };
+
+/* Per-head RMS norm of queries and keys and their position rotation, in one pass over the fused
+ * QKV projection (and, in the _quantize form, the per-token INT8 quantiser of all three):
+ *   y = x * rsqrt(mean(x^2) + eps) * w          per (token, head); no norm when the weights are NULL
+ *   (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)   over the first rotary_dim channels, pairs
+ *       (d, d + rotary_dim/2), or (2i, 2i+1) when `interleaved`; no rotation when positions and
+ *       the table are NULL
+ * in fp32 with one rounding at the end.
+ *   qkv        [tokens] rows of (heads + 2*kv_heads)*head_dim values, row_stride values apart:
+ *              query heads, key heads, value heads
+ *   q_weight, k_weight  fp32 [head_dim], both or neither
+ *   positions  int32 [tokens] (device); rope_table fp32 [rope_rows, rotary_dim]: the cosines of
+ *              the rotary_dim/2 frequencies, then their sines.  A position outside
+ *              [0, rope_rows) turns the rotated rows of its token into NaN (scales, when quantised).
+ *   out        [tokens, heads + kv_heads, head_dim], qkv's type (value heads are not copied)
+ *   codes      int8 [tokens, heads + 2*kv_heads, head_dim], scales fp32 [tokens, heads + 2*kv_heads]:
+ *              max(absmax, 1e-8)/127 and rne(y/scale), as i8tk_quantize_per_token_f32 gives for y
+ *   k_out      [tokens, kv_heads, head_dim] of qkv's type or NULL: the keys unquantised as well (for
+ *              i8tk_kv4_append)
+ * head_dim 64, 128 or 256; rotary_dim a multiple of 16, at most head_dim; row_stride a multiple of
+ * 8; all pointers except positions and scales 16-byte aligned. */
+int i8tk_qk_norm_rope(const void* qkv, int dtype, int64_t row_stride, const float* q_weight, const float* k_weight,
+                      const int32_t* positions, const float* rope_table, int rope_rows, int rotary_dim,
+                      int interleaved, float eps, void* out, int64_t tokens, int heads, int kv_heads, int head_dim,
+                      i8tk_stream_t stream);
+int i8tk_qk_norm_rope_quantize(const void* qkv, int dtype, int64_t row_stride, const float* q_weight,
+                               const float* k_weight, const int32_t* positions, const float* rope_table,
+                               int rope_rows, int rotary_dim, int interleaved, float eps, int8_t* codes,
+                               float* scales, void* k_out, int64_t tokens, int heads, int kv_heads, int head_dim,
+                               i8tk_stream_t stream);
+
+/* A paged key/value cache held in 4 bits: a pool of [num_pages][kv_heads] blocks, each one page of
+ * one key head, i8tk_kv4_block_bytes(page_size, head_dim) = page_size * (head_dim + head_dim/8) bytes:
+ *   keys' codes [page][D/2], values' codes [page][D/2],
+ *   keys' pairs [page][D/64] x {scale, centre} fp16, values' pairs likewise.
+ * A value is scale * (code - 8) + centre; per 64 channels of a row scale = fp16((max - min)/15),
+ * centre = fp16(min + 8*scale), code = clamp(rne((x - centre)/scale) + 8, 0, 15).  In a row 32-bit word
+ * u*(D/64) + g holds channels 64g + 8u .. 64g + 8u + 7, lowest nibble first.
+ *
+ * i8tk_kv4_append quantises new rows straight into the pool: k_new, v_new [tokens] rows of
+ * kv_heads*head_dim values of `dtype`, k_stride / v_stride values apart (so they may be slices of a
+ * fused projection); slots int64 [tokens] (device): page id * page_size + position in the page.  A
+ * slot outside the pool is skipped (-1 marks a padding row); the slots of a call are distinct.
+ * Values outside the fp16 range saturate; a NaN leaves unspecified codes in its group.
+ * i8tk_kv4_dequantize reads rows back: k, v fp16 [tokens, kv_heads, head_dim], zeros for a slot
+ * outside the pool.
+ * head_dim 64 or 128; page_size 16, 32, 64 or 128; pool, rows and outputs 16-byte aligned, strides
+ * multiples of 8. */
+int64_t i8tk_kv4_block_bytes(int page_size, int head_dim);
+int i8tk_kv4_append(const void* k_new, const void* v_new, int dtype, int64_t k_stride, int64_t v_stride, void* pool,
+                    const int64_t* slots, int64_t tokens, int kv_heads, int head_dim, int page_size,
+                    int64_t num_pages, i8tk_stream_t stream);
+int i8tk_kv4_dequantize(const void* pool, const int64_t* slots, void* k_f16, void* v_f16, int64_t tokens,
+                        int kv_heads, int head_dim, int page_size, int64_t num_pages, i8tk_stream_t stream);
+
+/* Decode attention (one query token per request) over that cache.
+ *   Q    int8 [batch] rows of heads*head_dim codes, q_stride apart; sQ fp32 [batch] rows of `heads`
+ *        scales, sq_stride apart (slices of i8tk_qk_norm_rope_quantize's outputs fit)
+ *   page_table int32 [batch, max_pages_per_seq], seq_lens int32 [batch] (device) as
+ *        i8tk_decode_attention_paged_checked: a length is read inside [0, max_seq_len], a page id outside
+ *        [0, num_pages) is not followed and recorded in the status block, a request of length 0
+ *        gets zeros
+ *   out  fp16 [batch, heads, head_dim]
+ * heads a multiple of kv_heads, at most 16 times as many; head_dim 64 or 128; page_size 16, 32, 64
+ * or 128; q_stride a multiple of 16; Q, pool and out 16-byte aligned; workspace 256-byte aligned. */
+size_t i8tk_decode_kv4_workspace_bytes(int batch, int heads, int kv_heads, int max_seq_len, int head_dim);
+int i8tk_decode_attention_kv4(const int8_t* Q, int64_t q_stride, const float* sQ, int64_t sq_stride,
+                              const void* pool, const int32_t* page_table, const int32_t* seq_lens, void* out_f16,
+                              int batch, int heads, int kv_heads, int max_seq_len, int page_size,
+                              int max_pages_per_seq, int head_dim, int64_t num_pages, void* workspace,
+                              size_t workspace_bytes, i8tk_stream_t stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

@@ -25,6 +25,9 @@ MLP_REFERENCE_ROUNDING = 8
 MLP_STATIC_SCALES = 16
 MLP_WORKSPACE_KEPT = 32
 
+F16 = 0
+BF16 = 1
+
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
@@ -69,6 +72,14 @@ SIGNATURES = {
     "i8tk_mlp_forward": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                               _i, _i, _i, _i, _vp, _sz, _vp]),
     "i8tk_linear_i8_f16": (_i, [_vp] * 6 + [_i] * 4 + [_vp, _sz, _vp]),
+    "i8tk_qk_norm_rope": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _i64, _i, _i, _i, _vp]),
+    "i8tk_qk_norm_rope_quantize": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _vp, _i64,
+                                        _i, _i, _i, _vp]),
+    "i8tk_kv4_block_bytes": (_i64, [_i, _i]),
+    "i8tk_kv4_append": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _vp, _i64, _i, _i, _i, _i64, _vp]),
+    "i8tk_kv4_dequantize": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i64, _vp]),
+    "i8tk_decode_kv4_workspace_bytes": (_sz, [_i] * 5),
+    "i8tk_decode_attention_kv4": (_i, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp] + [_i] * 7 + [_i64, _vp, _sz, _vp]),
     "i8tk_transpose_int8_weights": (_i, [_vp, _vp, _vp, _vp, _i, _i, _vp]),
 }
 

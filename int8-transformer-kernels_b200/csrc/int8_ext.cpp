@@ -460,6 +460,7 @@ void kv_append_quantize_torch(torch::Tensor k_new, torch::Tensor v_new, torch::T
 }  // namespace
 
 #include "int8_ext_mlp.inc"
+#include "int8_ext_grouped.inc"
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("int8_attention_forward", &int8_attention_forward_torch,
@@ -488,4 +489,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("check_status", &check_status_torch,
           "Synchronise the streams the ops ran on and raise if a bounded device-side wait gave up since the last check");
     register_mlp_ops(m);
+    register_grouped_ops(m);
 }

@@ -1,0 +1,223 @@
+// Writing rows into the 4-bit paged cache, and reading them back (layout: kv4.cuh).
+//
+//   per 64 channels:  scale  = fp16((max - min) / 15)
+//                     centre = fp16(min + 8 * scale)
+//                     code   = clamp(rne((x - centre) / scale), -8, 7) + 8       (scale 0: code 8)
+//
+// Every step is one IEEE operation in fp32 on 16-bit inputs, so the result does not depend on the order of anything.
+//
+// Bound by memory: 2 bytes read and 9/16 written per channel (read back: the other way round).  Eight lanes hold a
+// group of 64 channels, one 16-byte load each; minimum and maximum are three shuffles, a lane's eight codes are
+// exactly one word of the row.  A thread takes the key row and the value row of a token together.
+#include "kv4.cuh"
+
+#include <cuda_bf16.h>
+
+namespace i8tk {
+namespace {
+
+constexpr int kThreads = 128;
+
+__device__ __forceinline__ float2 widen(const __half*, uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+__device__ __forceinline__ float2 widen(const __nv_bfloat16*, uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Codes and pair of the eight channels of this lane in its group of eight lanes.
+template <typename T>
+__device__ __forceinline__ uint32_t quantize8(uint4 raw, __half2& pair) {
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    float x[8];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float2 v = widen(static_cast<const T*>(nullptr), w[k]);
+        // the pair is fp16: what lies outside its range saturates
+        x[2 * k] = fminf(fmaxf(v.x, -65504.f), 65504.f), x[2 * k + 1] = fminf(fmaxf(v.y, -65504.f), 65504.f);
+    }
+    float lo = x[0], hi = x[0];
+#pragma unroll
+    for (int k = 1; k < 8; ++k) lo = fminf(lo, x[k]), hi = fmaxf(hi, x[k]);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
+    }
+    const __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+    const float s = __half2float(sh);
+    const __half zh = __float2half_rn(__fadd_rn(lo, 8.0f * s));
+    const float z = __half2float(zh);
+    pair = __halves2half2(sh, zh);
+    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+    uint32_t word = 0;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float d = __fsub_rn(x[k], z);
+        const float t = d * inv;                     // within a few ulps of the quotient: only next to a tie is it divided
+        float r = rintf(t);
+        if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(d, s));
+        word |= (uint32_t)((int)fminf(fmaxf(r, -8.f), 7.f) + 8) << (4 * k);
+    }
+    return word;
+}
+
+// Where row (slot, head) lives: its block, and its position in the page; null when the slot is outside the pool.
+__device__ __forceinline__ unsigned char* block_of(unsigned char* pool, long long slot, long long slots, int page_shift, int kv_heads,
+                                                   int h, int block_bytes, int& at) {
+    if (slot < 0 || slot >= slots) return nullptr;
+    at = (int)(slot & ((1 << page_shift) - 1));
+    return pool + ((slot >> page_shift) * kv_heads + h) * (long long)block_bytes;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads)
+kv4_append_kernel(const T* __restrict__ k, const T* __restrict__ v, long long k_stride, long long v_stride,
+                  unsigned char* __restrict__ pool, const long long* __restrict__ slots, long long num_slots, int page_shift,
+                  long long rows, int kv_heads) {
+    constexpr int G = D / 64, LPR = D / 8;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int page = 1 << page_shift;
+    const int block_bytes = kv4_block_bytes(page, D);
+    const int sub = threadIdx.x % LPR, g = sub >> 3, u = sub & 7;
+    const long long row = ((long long)blockIdx.x * kThreads + threadIdx.x) / LPR;
+    const bool there = row < rows;
+    const long long t = there ? row / kv_heads : 0;
+    const int h = there ? (int)(row - t * kv_heads) : 0;
+    uint4 kr = make_uint4(0u, 0u, 0u, 0u), vr = kr;
+    int at = 0;
+    unsigned char* block = nullptr;
+    if (there) {
+        block = block_of(pool, slots[t], num_slots, page_shift, kv_heads, h, block_bytes, at);
+        kr = *reinterpret_cast<const uint4*>(k + t * k_stride + h * D + sub * 8);
+        vr = *reinterpret_cast<const uint4*>(v + t * v_stride + h * D + sub * 8);
+    }
+    __half2 kp, vp;
+    const uint32_t kw = quantize8<T>(kr, kp), vw = quantize8<T>(vr, vp);
+    if (block == nullptr) return;
+    unsigned char* codes = block + at * kv4_row_bytes(D) + (u * G + g) * 4;
+    *reinterpret_cast<uint32_t*>(codes) = kw;
+    *reinterpret_cast<uint32_t*>(codes + page * kv4_row_bytes(D)) = vw;
+    if (u == 0) {
+        __half2* pairs = reinterpret_cast<__half2*>(block + page * D) + at * G + g;
+        pairs[0] = kp;
+        pairs[page * G] = vp;
+    }
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads)
+kv4_dequantize_kernel(const unsigned char* __restrict__ pool, const long long* __restrict__ slots, long long num_slots,
+                      int page_shift, __half* __restrict__ k, __half* __restrict__ v, long long rows, int kv_heads) {
+    constexpr int G = D / 64, LPR = D / 8;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int page = 1 << page_shift;
+    const int sub = threadIdx.x % LPR, g = sub >> 3, u = sub & 7;
+    const long long row = ((long long)blockIdx.x * kThreads + threadIdx.x) / LPR;
+    if (row >= rows) return;
+    const long long t = row / kv_heads;
+    const int h = (int)(row - t * kv_heads);
+    int at = 0;
+    const unsigned char* block = block_of(const_cast<unsigned char*>(pool), slots[t], num_slots, page_shift, kv_heads, h,
+                                          kv4_block_bytes(page, D), at);
+    uint32_t w[2] = {0u, 0u};
+    float2 pair[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    if (block != nullptr) {
+        const unsigned char* codes = block + at * kv4_row_bytes(D) + (u * G + g) * 4;
+        const __half2* pairs = reinterpret_cast<const __half2*>(block + page * D) + at * G + g;
+        w[0] = *reinterpret_cast<const uint32_t*>(codes);
+        w[1] = *reinterpret_cast<const uint32_t*>(codes + page * kv4_row_bytes(D));
+        pair[0] = __half22float2(pairs[0]);
+        pair[1] = __half22float2(pairs[page * G]);
+    }
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+        uint32_t o[4];
+#pragma unroll
+        for (int k2 = 0; k2 < 4; ++k2) {
+            const float a = fmaf((float)((int)((w[m] >> (8 * k2)) & 15u) - 8), pair[m].x, pair[m].y);
+            const float b = fmaf((float)((int)((w[m] >> (8 * k2 + 4)) & 15u) - 8), pair[m].x, pair[m].y);
+            // the top code of a group that reaches the end of the fp16 range may lie half a step beyond it
+            const __half2 r = __floats2half2_rn(fminf(fmaxf(a, -65504.f), 65504.f), fminf(fmaxf(b, -65504.f), 65504.f));
+            o[k2] = *reinterpret_cast<const uint32_t*>(&r);
+        }
+        *reinterpret_cast<uint4*>((m == 0 ? k : v) + row * D + sub * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+}
+
+int check_kv4(const void* pool, const int64_t* slots, int64_t tokens, int kv_heads, int head_dim, int page_size, int64_t num_pages) {
+    I8TK_REQUIRE(pool && slots, I8TK_ERR_INVALID_ARGUMENT, "null pointer argument");
+    I8TK_REQUIRE(tokens > 0 && kv_heads > 0 && num_pages > 0, I8TK_ERR_INVALID_ARGUMENT, "sizes must be positive");
+    I8TK_REQUIRE(head_dim == 64 || head_dim == 128, I8TK_ERR_UNSUPPORTED, "head_dim must be 64 or 128 (got %d)", head_dim);
+    I8TK_REQUIRE(kv4_page_ok(page_size), I8TK_ERR_UNSUPPORTED, "page_size must be 16, 32, 64 or 128 (got %d)", page_size);
+    I8TK_REQUIRE(tokens < (1ll << 31) && num_pages < (1ll << 31) && kv_heads < (1 << 16) &&
+                     tokens * kv_heads * (head_dim / 8) / kThreads < (1ll << 31) - 1,
+                 I8TK_ERR_UNSUPPORTED, "too many rows");
+    I8TK_REQUIRE(aligned_to(pool, 16), I8TK_ERR_ALIGNMENT, "the pool must be 16-byte aligned");
+    return I8TK_OK;
+}
+
+int shift_of(int page) { return page == 16 ? 4 : page == 32 ? 5 : page == 64 ? 6 : 7; }
+
+template <typename T>
+int launch_append(const void* k, const void* v, int64_t ks, int64_t vs, void* pool, const int64_t* slots, int64_t tokens,
+                  int kv_heads, int D, int page, int64_t num_pages, cudaStream_t st) {
+    const long long rows = tokens * kv_heads, blocks = (rows * (D / 8) + kThreads - 1) / kThreads;
+    const dim3 grid((unsigned)blocks), block(kThreads);
+    if (D == 64)
+        I8TK_CUDA(launch_after(kv4_append_kernel<T, 64>, grid, block, 0, st, static_cast<const T*>(k), static_cast<const T*>(v), ks, vs,
+                               static_cast<unsigned char*>(pool), reinterpret_cast<const long long*>(slots), num_pages * page,
+                               shift_of(page), rows, kv_heads));
+    else
+        I8TK_CUDA(launch_after(kv4_append_kernel<T, 128>, grid, block, 0, st, static_cast<const T*>(k), static_cast<const T*>(v), ks, vs,
+                               static_cast<unsigned char*>(pool), reinterpret_cast<const long long*>(slots), num_pages * page,
+                               shift_of(page), rows, kv_heads));
+    return I8TK_OK;
+}
+
+}  // namespace
+}  // namespace i8tk
+
+using namespace i8tk;
+
+extern "C" int64_t i8tk_kv4_block_bytes(int page_size, int head_dim) {
+    if (!kv4_page_ok(page_size) || (head_dim != 64 && head_dim != 128)) return 0;
+    return kv4_block_bytes(page_size, head_dim);
+}
+
+extern "C" int i8tk_kv4_append(const void* k_new, const void* v_new, int dtype, int64_t k_stride, int64_t v_stride, void* pool,
+                               const int64_t* slots, int64_t tokens, int kv_heads, int head_dim, int page_size,
+                               int64_t num_pages, i8tk_stream_t stream) {
+    const int rc = check_kv4(pool, slots, tokens, kv_heads, head_dim, page_size, num_pages);
+    if (rc != I8TK_OK) return rc;
+    I8TK_REQUIRE(k_new && v_new, I8TK_ERR_INVALID_ARGUMENT, "null pointer argument");
+    I8TK_REQUIRE(dtype == I8TK_F16 || dtype == I8TK_BF16, I8TK_ERR_INVALID_ARGUMENT, "dtype must be I8TK_F16 or I8TK_BF16");
+    I8TK_REQUIRE(k_stride >= (int64_t)kv_heads * head_dim && v_stride >= (int64_t)kv_heads * head_dim && k_stride % 8 == 0 &&
+                     v_stride % 8 == 0,
+                 I8TK_ERR_INVALID_ARGUMENT, "token strides must cover a token's heads and be multiples of 8");
+    I8TK_REQUIRE(aligned_to(k_new, 16) && aligned_to(v_new, 16), I8TK_ERR_ALIGNMENT, "k_new and v_new must be 16-byte aligned");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (dtype == I8TK_F16)
+        return launch_append<__half>(k_new, v_new, k_stride, v_stride, pool, slots, tokens, kv_heads, head_dim, page_size, num_pages, st);
+    return launch_append<__nv_bfloat16>(k_new, v_new, k_stride, v_stride, pool, slots, tokens, kv_heads, head_dim, page_size, num_pages, st);
+}
+
+extern "C" int i8tk_kv4_dequantize(const void* pool, const int64_t* slots, void* k_f16, void* v_f16, int64_t tokens, int kv_heads,
+                                   int head_dim, int page_size, int64_t num_pages, i8tk_stream_t stream) {
+    const int rc = check_kv4(pool, slots, tokens, kv_heads, head_dim, page_size, num_pages);
+    if (rc != I8TK_OK) return rc;
+    I8TK_REQUIRE(k_f16 && v_f16, I8TK_ERR_INVALID_ARGUMENT, "null pointer argument");
+    I8TK_REQUIRE(aligned_to(k_f16, 16) && aligned_to(v_f16, 16), I8TK_ERR_ALIGNMENT, "k and v must be 16-byte aligned");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const long long rows = tokens * kv_heads, blocks = (rows * (head_dim / 8) + kThreads - 1) / kThreads;
+    const dim3 grid((unsigned)blocks), block(kThreads);
+    const unsigned char* p = static_cast<const unsigned char*>(pool);
+    const long long* sl = reinterpret_cast<const long long*>(slots);
+    if (head_dim == 64)
+        I8TK_CUDA(launch_after(kv4_dequantize_kernel<64>, grid, block, 0, st, p, sl, num_pages * page_size, shift_of(page_size),
+                               static_cast<__half*>(k_f16), static_cast<__half*>(v_f16), rows, kv_heads));
+    else
+        I8TK_CUDA(launch_after(kv4_dequantize_kernel<128>, grid, block, 0, st, p, sl, num_pages * page_size, shift_of(page_size),
+                               static_cast<__half*>(k_f16), static_cast<__half*>(v_f16), rows, kv_heads));
+    return I8TK_OK;
+}
