@@ -438,6 +438,26 @@ int i8tk_qk_norm_rope_quantize(const void* qkv, int dtype, int64_t row_stride, c
                                float* scales, void* k_out, int64_t tokens, int heads, int kv_heads, int head_dim,
                                i8tk_stream_t stream);
 
+/* INT8 attention over packed sequences of different lengths with grouped heads, causal or not.
+ *   Q [tokens] rows of heads*head_dim codes, K, V [tokens] rows of kv_heads*head_dim codes; sQ [tokens]
+ *   rows of `heads` scales (not negative), sK, sV [tokens] rows of kv_heads scales.  The strides are
+ *   elements between the rows of two tokens, so slices of i8tk_qk_norm_rope_quantize's outputs fit.
+ *   cu_seqlens int32 [batch + 1] (device): sequence b is rows cu_seqlens[b] .. cu_seqlens[b+1]; sequences
+ *   may be empty.  Entries are read inside [0, tokens]; a sequence longer than max_seqlen is cut to it.
+ *   out fp16 [tokens, heads, head_dim]; rows of no sequence (and behind a cut) are zero.
+ * score[i][j] = (q_i.k_j) * sQ_i * sK_j / sqrt(D) for the j of i's sequence (j <= i when causal); what the
+ * other positions hold, NaN and infinities included, does not reach the row.  A value scale that is
+ * not finite makes the rows that see it NaN.
+ * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 64 times as many; strides of Q, K,
+ * V multiples of 16; Q, K, V and out 16-byte aligned; workspace
+ * i8tk_attention_varlen_workspace_bytes(...) bytes, 256-byte aligned. */
+size_t i8tk_attention_varlen_workspace_bytes(int64_t tokens, int batch, int heads, int kv_heads, int head_dim);
+int i8tk_attention_varlen(const int8_t* Q, int64_t q_stride, const int8_t* K, int64_t k_stride, const int8_t* V,
+                          int64_t v_stride, const float* sQ, int64_t sq_stride, const float* sK, int64_t sk_stride,
+                          const float* sV, int64_t sv_stride, const int32_t* cu_seqlens, void* out_f16,
+                          int64_t tokens, int batch, int max_seqlen, int heads, int kv_heads, int head_dim, int causal,
+                          void* workspace, size_t workspace_bytes, i8tk_stream_t stream);
+
 /* A paged key/value cache held in 4 bits: a pool of [num_pages][kv_heads] blocks, each one page of
  * one key head, i8tk_kv4_block_bytes(page_size, head_dim) = page_size * (head_dim + head_dim/8) bytes:
  *   keys' codes [page][D/2], values' codes [page][D/2],

@@ -75,6 +75,8 @@ SIGNATURES = {
     "i8tk_qk_norm_rope": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _i64, _i, _i, _i, _vp]),
     "i8tk_qk_norm_rope_quantize": (_i, [_vp, _i, _i64, _vp, _vp, _vp, _vp, _i, _i, _i, _f, _vp, _vp, _vp, _i64,
                                         _i, _i, _i, _vp]),
+    "i8tk_attention_varlen_workspace_bytes": (_sz, [_i64, _i, _i, _i, _i]),
+    "i8tk_attention_varlen": (_i, [_vp, _i64] * 6 + [_vp, _vp, _i64] + [_i] * 6 + [_vp, _sz, _vp]),
     "i8tk_kv4_block_bytes": (_i64, [_i, _i]),
     "i8tk_kv4_append": (_i, [_vp, _vp, _i, _i64, _i64, _vp, _vp, _i64, _i, _i, _i, _i64, _vp]),
     "i8tk_kv4_dequantize": (_i, [_vp, _vp, _vp, _vp, _i64, _i, _i, _i, _i64, _vp]),

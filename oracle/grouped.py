@@ -112,14 +112,15 @@ def int4_decode(q, sq, keys, values):
 def varlen_attention(q, k, v, sq, sk, sv, cu, causal=True):
     """Packed INT8 attention: q [T, H, D], k, v [T, kv, D] codes, scales per row.  Returns (out [T, H, D], bound):
     half a step of every fp16 p * scale (2^-11 of the sum of p |v|) and of the fp16 result, with 5 % for the fp32
-    parts and, for products below the fp16 range, 2^-29 of the sequence's largest |v| for each key (p * scale is
-    scaled so that the largest scale of the sequence is at least 2^6, and half the smallest fp16 number is 2^-25)."""
+    parts; for products below the fp16 range 2^-31 of the sequence's largest |v| for each key (p * scale is scaled
+    so that the largest scale of the sequence is at least 2^6, and half the smallest fp16 number is 2^-25); and for
+    the three fp32 roundings of a score s, which move its probability by 3 * 2^-24 * |s| and the sum by as much."""
     T, H, D = q.shape
     kv = k.shape[1]
     out, bound = np.zeros((T, H, D)), np.zeros((T, H, D))
     for a, b in zip(cu[:-1], cu[1:]):
         n = b - a
-        for h in range(kv):
+        for h in range(kv if n > 0 else 0):
             at = slice(h * (H // kv), (h + 1) * (H // kv))
             qf = q[a:b, at].astype(np.float64) * sq[a:b, at, None].astype(np.float64)
             kf = k[a:b, h].astype(np.float64) * sk[a:b, h, None].astype(np.float64)
@@ -130,7 +131,9 @@ def varlen_attention(q, k, v, sq, sk, sv, cu, causal=True):
             p, l = softmax_rows(s)
             o = np.einsum("gij,jd->gid", p / l, vf)
             spread = np.einsum("gij,jd->gid", p / l, np.abs(vf))
-            tiny = 2.0 ** -25 * n * 127 * float(sv[a:b, h].max()) / 64 * 256 / l if n else 0.0
+            size = np.abs(np.where(np.isfinite(s), s, 0.0)).max(-1, keepdims=True)
+            tiny = 2.0 ** -25 * n * 127 * float(sv[a:b, h].max()) / 64 / l
             out[a:b, at] = o.transpose(1, 0, 2)
-            bound[a:b, at] = (1.05 * (2.0 ** -11 * (spread + np.abs(o)) + tiny + 2.0 ** -25)).transpose(1, 0, 2)
+            step = 2.0 ** -11 + 3 * 2.0 ** -24 * size
+            bound[a:b, at] = (1.05 * (step * (spread + np.abs(o)) + tiny + 2.0 ** -25)).transpose(1, 0, 2)
     return out, bound
