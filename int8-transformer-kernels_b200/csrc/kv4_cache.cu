@@ -22,40 +22,74 @@ __device__ __forceinline__ float2 widen(const __half*, uint32_t v) { return __ha
 __device__ __forceinline__ float2 widen(const __nv_bfloat16*, uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
 }
+// minimum of the pairs in two words; the sign bits of a word flipped
+__device__ __forceinline__ uint32_t min2(const __half*, uint32_t a, uint32_t b) {
+    const __half2 m = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+__device__ __forceinline__ uint32_t min2(const __nv_bfloat16*, uint32_t a, uint32_t b) {
+    const __nv_bfloat162 m = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+}
+// x / 15 correctly rounded: a quotient from the rounded reciprocal, corrected by its exact remainder (Markstein)
+__device__ __forceinline__ float div15(float x) {
+    const float r = 1.0f / 15.0f;
+    const float q = x * r;
+    return fmaf(fmaf(-15.0f, q, x), r, q);
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // Codes and pair of the eight channels of this lane in its group of eight lanes.
 template <typename T>
 __device__ __forceinline__ uint32_t quantize8(uint4 raw, __half2& pair) {
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-    float x[8];
+    const T* tag = nullptr;
+    constexpr uint32_t kSigns = 0x80008000u;
+    // minimum of the values and of their negatives, both as 16-bit numbers: exact, and one word to shuffle
+    const uint32_t lo2 = min2(tag, min2(tag, raw.x, raw.y), min2(tag, raw.z, raw.w));
+    const uint32_t hi2 = min2(tag, min2(tag, raw.x ^ kSigns, raw.y ^ kSigns), min2(tag, raw.z ^ kSigns, raw.w ^ kSigns));
+    uint32_t both = min2(tag, prmt(lo2, hi2, 0x5410u), prmt(lo2, hi2, 0x7632u));
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const float2 v = widen(static_cast<const T*>(nullptr), w[k]);
-        // the pair is fp16: what lies outside its range saturates
-        x[2 * k] = fminf(fmaxf(v.x, -65504.f), 65504.f), x[2 * k + 1] = fminf(fmaxf(v.y, -65504.f), 65504.f);
-    }
-    float lo = x[0], hi = x[0];
-#pragma unroll
-    for (int k = 1; k < 8; ++k) lo = fminf(lo, x[k]), hi = fmaxf(hi, x[k]);
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    }
-    const __half sh = __float2half_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f));
+    for (int o = 4; o > 0; o >>= 1) both = min2(tag, both, __shfl_xor_sync(0xffffffffu, both, o));
+    // the pair is fp16: a range that does not fit saturates
+    const float lo = fminf(fmaxf(widen(tag, both).x, -65504.f), 65504.f), hi = fminf(fmaxf(-widen(tag, both).y, -65504.f), 65504.f);
+    const __half sh = __float2half_rn(div15(__fsub_rn(hi, lo)));
     const float s = __half2float(sh);
     const __half zh = __float2half_rn(__fadd_rn(lo, 8.0f * s));
     const float z = __half2float(zh);
     pair = __halves2half2(sh, zh);
-    const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-    uint32_t word = 0;
+    const float inv = s > 0.f ? rcp_approx(s) : 0.f;
+    const f32x2 inv2 = pack2(inv, inv), nz2 = pack2(-z, -z);
+    // code + 8 in the low bits of 1.5 * 2^23 + 8 + (x - z) / s; the product with the approximate reciprocal is within
+    // a few ulps of the quotient, so only next to a tie is it divided
+    const f32x2 magic = pack2(12582920.f, 12582920.f), unmagic = pack2(-12582920.f, -12582920.f);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+    f32x2 d[4], q[4];
+    float off = 0.f;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-        const float d = __fsub_rn(x[k], z);
-        const float t = d * inv;                     // within a few ulps of the quotient: only next to a tie is it divided
-        float r = rintf(t);
-        if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(d, s));
-        word |= (uint32_t)((int)fminf(fmaxf(r, -8.f), 7.f) + 8) << (4 * k);
+    for (int k = 0; k < 4; ++k) {
+        d[k] = add2(widen(tag, w[k]), nz2);
+        const f32x2 t = mul2(d[k], inv2);
+        // far outside (saturated inputs) the sum would leave the magic number's range
+        q[k] = add2(pack2(fminf(fmaxf(t.x, -64.f), 64.f), fminf(fmaxf(t.y, -64.f), 64.f)), magic);
+        const f32x2 n = add2(q[k], unmagic), e = add2(t, pack2(-n.x, -n.y));
+        off = max3(off, fabsf(e.x), fabsf(e.y));
+    }
+    if (off > 0.4999f && s > 0.f) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            q[k] = pack2(fminf(fmaxf(rintf(__fdiv_rn(d[k].x, s)), -8.f), 7.f) + 12582920.f, fminf(fmaxf(rintf(__fdiv_rn(d[k].y, s)), -8.f), 7.f) + 12582920.f);
+    }
+    // channels e and e + 4 side by side in 16 bits each, clamped to 0..15, four nibbles apart
+    uint32_t word = 0;
+    const float qe[8] = {q[0].x, q[0].y, q[1].x, q[1].y, q[2].x, q[2].y, q[3].x, q[3].y};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        const uint32_t p = __vimin_s16x2_relu(prmt(__float_as_uint(qe[e]), __float_as_uint(qe[e + 4]), 0x5410u), 0x000f000fu);
+        word += p << (4 * e);
     }
     return word;
 }
@@ -121,27 +155,31 @@ kv4_dequantize_kernel(const unsigned char* __restrict__ pool, const long long* _
     const unsigned char* block = block_of(const_cast<unsigned char*>(pool), slots[t], num_slots, page_shift, kv_heads, h,
                                           kv4_block_bytes(page, D), at);
     uint32_t w[2] = {0u, 0u};
-    float2 pair[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+    __half2 pair[2] = {__floats2half2_rn(0.f, 0.f), __floats2half2_rn(0.f, 0.f)};
     if (block != nullptr) {
         const unsigned char* codes = block + at * kv4_row_bytes(D) + (u * G + g) * 4;
         const __half2* pairs = reinterpret_cast<const __half2*>(block + page * D) + at * G + g;
         w[0] = *reinterpret_cast<const uint32_t*>(codes);
         w[1] = *reinterpret_cast<const uint32_t*>(codes + page * kv4_row_bytes(D));
-        pair[0] = __half22float2(pairs[0]);
-        pair[1] = __half22float2(pairs[page * G]);
+        pair[0] = pairs[0];
+        pair[1] = pairs[page * G];
     }
+    const __half2 bias = __floats2half2_rn(1032.f, 1032.f), top = __floats2half2_rn(65504.f, 65504.f), bottom = __floats2half2_rn(-65504.f, -65504.f);
 #pragma unroll
     for (int m = 0; m < 2; ++m) {
-        uint32_t o[4];
+        const __half2 s = __low2half2(pair[m]), z = __high2half2(pair[m]);
+        uint32_t v4[4];                              // channels e and e + 4
 #pragma unroll
-        for (int k2 = 0; k2 < 4; ++k2) {
-            const float a = fmaf((float)((int)((w[m] >> (8 * k2)) & 15u) - 8), pair[m].x, pair[m].y);
-            const float b = fmaf((float)((int)((w[m] >> (8 * k2 + 4)) & 15u) - 8), pair[m].x, pair[m].y);
-            // the top code of a group that reaches the end of the fp16 range may lie half a step beyond it
-            const __half2 r = __floats2half2_rn(fminf(fmaxf(a, -65504.f), 65504.f), fminf(fmaxf(b, -65504.f), 65504.f));
-            o[k2] = *reinterpret_cast<const uint32_t*>(&r);
+        for (int e = 0; e < 4; ++e) {                // 1024 + code as a half, less 1032: exact
+            const uint32_t c = ((w[m] >> (4 * e)) & 0x000f000fu) | 0x64006400u;
+            // one rounding, of scale * (code - 8) + centre; the top code of a group that reaches the end of the fp16
+            // range may lie half a step beyond it
+            __half2 x = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&c), bias), s, z);
+            x = __hmax2(__hmin2(x, top), bottom);
+            v4[e] = *reinterpret_cast<const uint32_t*>(&x);
         }
-        *reinterpret_cast<uint4*>((m == 0 ? k : v) + row * D + sub * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+        *reinterpret_cast<uint4*>((m == 0 ? k : v) + row * D + sub * 8) =
+            make_uint4(prmt(v4[0], v4[1], 0x5410u), prmt(v4[2], v4[3], 0x5410u), prmt(v4[0], v4[1], 0x7632u), prmt(v4[2], v4[3], 0x7632u));
     }
 }
 

@@ -18,11 +18,18 @@
 //   permute first, its 1/16 is applied to the accumulators at the end.
 // * The scores come out with positions as rows; the probabilities turn around for the second product with one
 //   8x8 transposing move per eight positions.
+// * With 4 heads or fewer in a group, the 8 columns are W = 2 or 4 copies of the heads, and copy w takes every W-th
+//   octet of positions: the products cost the same, but the work per score -- scales, exponentials, packing -- is done
+//   for one octet per lane instead of for W of which only one has heads in the lane.  A copy keeps a maximum and sums of
+//   its own, as a row apart, and the copies are merged with the warps' rows.
 //
 // The tiles (128 positions) of all (request, key head) rows, in that order, are one sequence, cut into equal runs for
 // the CTAs from the lengths on the device: a short request costs what it reads.  Every CTA adds the lengths up itself
-// (they are a few hundred words), so nothing runs ahead of the scan.  In a CTA one warp brings pages by bulk copies,
-// one copy per page and head, into a ring; four warps take 32 positions of a tile each and meet only where a row ends.
+// (they are a few hundred words), so nothing runs ahead of the scan.  A CTA is four warps, 32 positions of a tile each,
+// which meet only where a row ends; in turn they start the bulk copies of the next tile, one copy per page and head.
+// There is no warp for the copies alone: the unpacking is bound by the instructions the SM can issue, and four CTAs of
+// four 128-register warps are all it holds (with a fifth warp it held three).  The page size is a template parameter,
+// so that every shared-memory address is a constant off three per-thread bases.
 // A row that one CTA scans whole is written there; a row cut between CTAs leaves at most two partial rows per CTA,
 // merged by a second kernel that is launched behind the first one's tail.
 #include "kv4.cuh"
@@ -33,23 +40,29 @@ namespace i8tk {
 namespace {
 
 constexpr int kTile = 128;                  // positions
-constexpr int kWarps = 4;                   // scanning warps, 32 positions each
-constexpr int kScanThreads = (kWarps + 1) * 32;
-constexpr float kLazy = 2.0f;               // log2 units a row's maximum may run ahead of its reference: p <= 4, and
-                                            // 4 * (largest scale, 131008 / 15) is still an fp16 number
+constexpr int kWarps = 4;                   // 32 positions each
+constexpr int kScanThreads = kWarps * 32;
+// P = p * s has to stay an fp16 number (below 2^16) and should use its range: a row's reference lies kTop log2 units
+// below its largest score times the largest scale met so far, and moves when a product would run kSlack above that.
+constexpr float kTop = 13.0f, kSlack = 2.0f;
+constexpr int kLeastScale = -20;          // log2 of the scale assumed for values that have none (p itself stays below 2^35)
+constexpr float kNoReference = 1e30f;       // negative reference of a row that has met nothing: 2^(-inf + 1e30) is still 0
 
-template <int D, int NT>                    // NT: blocks of 8 query heads per key head
+template <int D, int NT, int W>             // NT: blocks of 8 query heads per key head; W: copies of the heads in a block
 struct Kv4Cfg {
     static constexpr int G = D / 64;
     static constexpr int TILE_BYTES = kTile * (D + D / 8);
-    static constexpr int STAGES = D == 64 ? 4 : 3;
-    static constexpr int CTAS = NT == 1 ? 3 : 2;                  // per SM
-    static constexpr int HEADS = NT * 8;
+    // Two stages: a third (32 requests, up to 32768 positions, 32/8 heads, D 128: 127 us a call waited for, against 134)
+    // fills the SM's shared memory, and a call that follows at once loses more (153 us against 122).
+    static constexpr int STAGES = 2;
+    static constexpr int CTAS = NT == 2 ? 3 : 4;                  // per SM: 168 and 128 registers a thread
     static constexpr int ROW = D + 4;                             // floats of a partial row: acc[D], m, l, -, -
-    static constexpr int OFF_MERGE = STAGES * TILE_BYTES;         // [kWarps][HEADS][ROW]
-    static constexpr int OFF_BARS = OFF_MERGE + kWarps * HEADS * ROW * 4;
+    static constexpr int OFF_BARS = STAGES * TILE_BYTES;
     static constexpr int SMEM = OFF_BARS + STAGES * 16;
-    static_assert(SMEM * CTAS <= 227 * 1024, "shared memory of an SM");
+    // where a row ends, the warps' rows of 8 columns meet in the stage just read
+    static_assert(kWarps * 8 * ROW * 4 <= TILE_BYTES, "a stage holds the rows of the warps");
+    static_assert(STAGES >= 2 && STAGES <= kWarps, "each of the first tiles has a warp of its own");
+    static_assert((SMEM + 1024 + 128) * CTAS <= 227 * 1024, "shared memory of an SM");
 };
 
 constexpr uint32_t kNotedBadIndex = 1u, kNotedTimeout = 2u;
@@ -62,7 +75,7 @@ struct Kv4Args {
     const int* table;                       // [B][max_pages]
     const int* lens;                        // [B]
     __half* out;                            // [B][heads][D]
-    int B, kv_heads, group, max_len, page_shift, max_pages, num_pages;
+    int B, kv_heads, group, max_len, max_pages, num_pages;
     float score_scale;                      // log2(e) / sqrt(D)
     uint32_t* status;
     int* prefix;                            // [B + 1] tiles per key head of the requests before
@@ -85,13 +98,18 @@ __device__ __forceinline__ long long run_start(long long total, int c, int n) { 
 __device__ __forceinline__ int run_owner(long long total, long long tile, int n) { return (int)(((tile + 1) * n - 1) / total); }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void mma_16816_from_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
     uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
     return r;
 }
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -99,45 +117,52 @@ __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 template <int W>
-__device__ __forceinline__ void lds_words(uint32_t addr, uint32_t (&w)[W]) {
-    if constexpr (W == 1) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(addr));
-    if constexpr (W == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-    if constexpr (W == 4)
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(addr));
+__device__ __forceinline__ void lds_words(const unsigned char* at, uint32_t (&w)[W]) {
+    if constexpr (W == 1) w[0] = *reinterpret_cast<const uint32_t*>(at);
+    if constexpr (W == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(at);
+        w[0] = v.x, w[1] = v.y;
+    }
+    if constexpr (W == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(at);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    }
 }
 __device__ __forceinline__ float2 pair_of(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
-// Position of the sequence of tiles: request, key head, tile of the row.
-struct Cursor {
-    int b, h, tile, tiles, len;
+// A row of the sequence: request, key head, tiles.
+struct Row {
+    int b, h, len, tiles;
 };
-__device__ __forceinline__ void load_row(const Kv4Args& a, Cursor& c) {
-    c.len = row_len(a, c.b);
-    c.tiles = (c.len + kTile - 1) / kTile;
+__device__ __forceinline__ void load_row(const Kv4Args& a, Row& r) {
+    r.len = row_len(a, r.b);
+    r.tiles = (r.len + kTile - 1) / kTile;
 }
-// to the next tile; called only while tiles remain, the bound on b is for lengths that changed under the kernel
-__device__ __forceinline__ void advance(const Kv4Args& a, Cursor& c) {
-    if (++c.tile < c.tiles) return;
-    c.tile = 0;
-    if (++c.h < a.kv_heads) return;
-    c.h = 0;
-    while (c.b + 1 < a.B) {
-        ++c.b;
-        load_row(a, c);
-        if (c.tiles > 0) return;
+// the next row that has tiles; called only while tiles remain, the bound on b (and the length it then gives) is for
+// lengths that changed under the kernel
+__device__ __forceinline__ void next_row(const Kv4Args& a, Row& r) {
+    if (++r.h < a.kv_heads) return;
+    r.h = 0;
+    while (r.b + 1 < a.B) {
+        ++r.b;
+        load_row(a, r);
+        if (r.tiles > 0) return;
     }
+    r.tiles = 1 << 30, r.len = 0;
 }
 
-template <int D, int NT>
-__global__ void __launch_bounds__(kScanThreads, Kv4Cfg<D, NT>::CTAS)
+template <int D, int NT, int W, int PAGE>
+__global__ void __launch_bounds__(kScanThreads, Kv4Cfg<D, NT, W>::CTAS)
 kv4_scan_kernel(const Kv4Args a) {
-    using Cfg = Kv4Cfg<D, NT>;
+    using Cfg = Kv4Cfg<D, NT, W>;
     constexpr int G = Cfg::G, ROW = Cfg::ROW;
+    constexpr int HEADS = 8 / W;             // query heads of a block of columns
+    constexpr int NU = W == 4 ? 1 : 2, NE = W == 1 ? 2 : 1;      // octets of 32 positions a lane has scores of: NU * NE
     extern __shared__ __align__(128) unsigned char smem[];
-    __shared__ int s_warp[kWarps + 1];
+    __shared__ int s_warp[kWarps];
     __shared__ int s_start[2];
     const uint32_t base = smem_u32(smem), bars = base + Cfg::OFF_BARS;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     auto full = [&](int s) { return bars + 16u * s; };
     auto empty = [&](int s) { return bars + 16u * s + 8u; };
     if (threadIdx.x == 0) {
@@ -166,7 +191,7 @@ kv4_scan_kernel(const Kv4Args a) {
     __syncthreads();
     int before = inc - mine, sum = 0;
 #pragma unroll
-    for (int w = 0; w <= kWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
         if (w < warp) before += s_warp[w];
         sum += s_warp[w];
     }
@@ -197,67 +222,62 @@ kv4_scan_kernel(const Kv4Args a) {
     if (threadIdx.x == 0) a.noted[blockIdx.x] = 0u;
     __syncthreads();
     if (run == 0) return;
-    Cursor cur;
+    Row cur;
     cur.b = s_start[0];
     load_row(a, cur);
+    int tile;                                // of the row
     {
         const long long in = first - (long long)s_start[1] * a.kv_heads;
         cur.h = (int)(in / max(cur.tiles, 1));
-        cur.tile = (int)(in - (long long)cur.h * cur.tiles);
+        tile = (int)(in - (long long)cur.h * cur.tiles);
     }
-    const int page = 1 << a.page_shift, block_bytes = kv4_block_bytes(page, D);
+    static_assert(kv4_block_bytes(PAGE, D) % D == 0 && Cfg::TILE_BYTES % D == 0, "rows pair up by one address bit");
+    constexpr int BLOCK = kv4_block_bytes(PAGE, D), PAGES = kTile / PAGE;      // pages of a tile: 1 to 8, a lane each
 
-    if (warp == kWarps) {
-        // ================= one warp brings the pages =================
-        const int per_tile = kTile >> a.page_shift;          // pages of a tile: 1 to 8, a lane each
-        bool ok = true;
-        int i = 0, bad = 0;
-        for (; i < run && ok; ++i) {
-            const int s = i % Cfg::STAGES;
-            const int p = cur.tile * per_tile + lane;
-            const bool use = lane < per_tile && p * page < cur.len;
-            int id = 0;
-            if (use) {
-                id = __ldg(a.table + (long long)cur.b * a.max_pages + p);
-                if ((unsigned)id >= (unsigned)a.num_pages) id = 0, ++bad;      // never followed
-            }
-            const int pages = __popc(__ballot_sync(0xffffffffu, use));
-            const bool got = mbar_wait_bounded(empty(s), ((i / Cfg::STAGES) & 1) ^ 1);
-            ok = __all_sync(0xffffffffu, got);
-            if (!ok) break;
-            if (lane == 0) mbar_expect_tx(full(s), pages * block_bytes);
-            __syncwarp();
-            if (use)
-                bulk_g2s(base + s * Cfg::TILE_BYTES + lane * block_bytes, a.pool + ((long long)id * a.kv_heads + cur.h) * block_bytes,
-                         block_bytes, full(s));
-            if (i + 1 < run) advance(a, cur);
+    // ---- copies: tile i of the run is brought by warp i % 4, a lane per page, STAGES - 1 tiles ahead ----
+    auto look_up = [&](const Row& r, int t) {
+        const int p = t * PAGES + lane;
+        return lane < PAGES && p * PAGE < r.len ? __ldg(a.table + (long long)r.b * a.max_pages + p) : 0;
+    };
+    // tile t counted from the start of row `r`, which may lie rows behind it
+    auto find = [&](Row& r, int& t) {
+        while (t >= r.tiles) {
+            t -= r.tiles;
+            next_row(a, r);
         }
-        if (!ok) {                           // copies still in flight land before this block lets go of its memory
-            if (lane == 0) note(a, kNotedTimeout, 1u);
-            for (int k = max(0, i - Cfg::STAGES); k < i; ++k) mbar_wait_bounded(full(k % Cfg::STAGES), (k / Cfg::STAGES) & 1, 64u);
+    };
+    auto issue = [&](const Row& r, int t, int id, int s) {       // tile t of row r, whose page ids the lanes hold, into stage s
+        const int left = max(r.len - t * kTile, 0);
+        if ((unsigned)id >= (unsigned)a.num_pages) {                           // never followed
+            id = 0;
+            note(a, kNotedBadIndex, 1u);
         }
-        bad = __reduce_add_sync(0xffffffffu, bad);
-        if (lane == 0 && bad > 0) note(a, kNotedBadIndex, (uint32_t)bad);
-        return;
-    }
+        if (lane == 0) mbar_expect_tx(full(s), (left >= kTile ? PAGES : (left + PAGE - 1) / PAGE) * BLOCK);
+        __syncwarp();
+        if (lane < PAGES && lane * PAGE < left)
+            bulk_g2s(base + s * Cfg::TILE_BYTES + lane * BLOCK, a.pool + ((long long)id * a.kv_heads + r.h) * BLOCK, BLOCK, full(s));
+    };
 
-    // ================= four warps scan, 32 positions of a tile each =================
     const int gid = lane >> 2, tig = lane & 3;
     const int row = gid ^ ((gid >> 1) & 1);                  // row gid of an operand holds this position of eight: the two
                                                              // lanes groups of a shared-memory phase then differ in parity
     const int vrow = (2 * tig) ^ (tig & 1);                  // the same order seen from the second product
-    float* merge = reinterpret_cast<float*>(smem + Cfg::OFF_MERGE);
     const int heads = a.kv_heads * a.group;
+    // this lane's octet among the two of 16 positions (W >= 2), and its 16 of the 32 (W = 4); the copy its operand rows
+    // of the second product belong to
+    const int my_e = W == 2 ? tig >> 1 : W == 4 ? tig & 1 : 0, my_u = W == 4 ? tig >> 1 : 0, copy = gid / HEADS;
 
     uint32_t q[NT][G * 2][4];                                // per word of a key row: code pairs (0,4) (1,5)/16 (2,6) (3,7)/16
     f32x2 to_log2[NT], qz[NT][G], q8[NT][G];                 // heads 2 tig, 2 tig + 1
     float acc[NT][G][4][4], ones[NT][G][4];
-    f32x2 m_ref[NT], l2[NT], w2[NT][G];
+    f32x2 neg[NT], l2[NT], w2[NT][G];                        // negative reference; sums of p and of p * centre
+    float top, room;                                         // a power of two no value scale met is above; how far a score
+                                                             // may be above the reference with it
 
     auto begin_row = [&]() {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
-            const int j = n * 8 + gid;                       // this lane's query head in the group
+            const int j = n * 8 + gid % HEADS;               // this lane's query head in the group
             const bool real = j < a.group;
             int sums[G];
 #pragma unroll
@@ -299,119 +319,190 @@ kv4_scan_kernel(const Kv4Args a) {
                 for (int k = 0; k < 4; ++k) ones[n][g][k] = 0.f;
                 w2[n][g] = pack2(0.f, 0.f);
             }
-            m_ref[n] = pack2(-INFINITY, -INFINITY);
+            neg[n] = pack2(kNoReference, kNoReference);
             l2[n] = pack2(0.f, 0.f);
         }
+        top = 1.0f / (1 << -kLeastScale);
+        room = kTop + kSlack - kLeastScale;
     };
 
-    bool ok = true;
-    int seg_first = cur.tile;                                // first tile of the row in this run
-    begin_row();
-    for (int i = 0; i < run; ++i) {
-        const int s = i % Cfg::STAGES;
-        if (ok) {
-            const bool got = mbar_wait_bounded(full(s), (i / Cfg::STAGES) & 1);
-            ok = __all_sync(0xffffffffu, got);
-            if (!ok && lane == 0) note(a, kNotedTimeout, 1u);
-        }
-        const int left = cur.len - cur.tile * kTile - warp * 32;     // positions of this warp's 32 that exist
-        if (ok && left > 0) {
+    int s = 0;
+    uint32_t phase = 0;
+    if (warp < min(Cfg::STAGES - 1, run)) {
+        Row r = cur;
+        int t = tile + warp;
+        find(r, t);
+        issue(r, t, look_up(r, t), warp);
+    }
+    // this thread's rows: keys at row `row` of its 16, values at row vrow, both of the warp's first 16 positions
+    constexpr int U = PAGE == 16 ? BLOCK : 16 * (D / 2), U_PAIRS = PAGE == 16 ? BLOCK : 16 * G * 4;     // to the next 16
+    const int p0 = warp * 32, in_page = p0 % PAGE;
+    const int warp_block = p0 / PAGE * BLOCK;
+    int k_at = warp_block + (in_page + row) * (D / 2) + tig * (D / 8);
+    int pair_at = warp_block + PAGE * D + (in_page + row + 8 * my_e) * (G * 4) + my_u * U_PAIRS;
+    int v_at = warp_block + PAGE * (D / 2) + (in_page + vrow) * (D / 2) + gid * (G * 4);
+    constexpr int PAIRS = PAGE * G * 4;                     // from the keys' pairs to the values'
+    auto next_stage = [&]() {
+        const bool wrap = s == Cfg::STAGES - 1;
+        const int to = wrap ? -(Cfg::STAGES - 1) * Cfg::TILE_BYTES : Cfg::TILE_BYTES;
+        k_at += to, pair_at += to, v_at += to;
+        phase ^= wrap ? 1u : 0u;
+        s = wrap ? 0 : s + 1;
+    };
+    for (int i = 0; i < run;) {              // a piece of a row: to its end, or to the end of the run
+        const int pieces = min(cur.tiles - tile, run - i), seg_first = tile;
+        const bool row_ends = tile + pieces == cur.tiles, more = i + pieces < run;
+        begin_row();
+        int left = cur.len - tile * kTile - warp * 32;           // positions of this warp's 32 that exist
+        int ahead_id = 0;                                        // page ids of this warp's next turn in this row
+        for (int k = 0; k < pieces; ++k, ++i, left -= kTile) {
+            // ---- the tile STAGES - 1 ahead, into the stage the last one was read from ----
+            if (((i + Cfg::STAGES - 1) & 3) == warp && i + Cfg::STAGES - 1 < run) {
+                const int o = s == 0 ? Cfg::STAGES - 1 : s - 1;
+                if (i > 0) {
+                    const bool got = mbar_wait_bounded(empty(o), s == 0 ? phase ^ 1 : phase);
+                    if (!__all_sync(0xffffffffu, got)) goto late;
+                }
+                int t = tile + k + Cfg::STAGES - 1;
+                if (t < cur.tiles) {
+                    issue(cur, t, k >= 4 ? ahead_id : look_up(cur, t), o);
+                    ahead_id = look_up(cur, t + 4);              // (behind the row's end: nothing)
+                } else {
+                    Row r = cur;
+                    find(r, t);
+                    issue(r, t, look_up(r, t), o);
+                }
+            }
+            {
+                const bool got = mbar_try_wait(full(s), phase);
+                if (!__all_sync(0xffffffffu, got)) {
+                    const bool at_last = mbar_wait_bounded(full(s), phase);
+                    if (!__all_sync(0xffffffffu, at_last)) goto late;
+                }
+            }
+            if (left > 0) {
             // ---- scores of 2 x 16 positions ----
-            f32x2 sc[2][2][NT];                              // [16 positions][row gid, gid + 8][8 heads]
-            uint32_t vp[2][2][G];                            // the values' pairs of the same positions
-            uint32_t blk[2];
+            f32x2 sc[NU][NE][NT];                            // [16 positions][row gid, gid + 8][8 columns]
+            uint32_t vp[NU][NE][G];                          // the values' pairs of the same positions
+            uint32_t wa[2][2 * G], wb[2][2 * G];
+            float dot[2][NT][G][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                const int p0 = warp * 32 + u * 16;
-                blk[u] = base + s * Cfg::TILE_BYTES + (p0 >> a.page_shift) * block_bytes;
-                const int r = (p0 & (page - 1)) + row;
-                uint32_t wa[2 * G], wb[2 * G];
-                lds_words(blk[u] + r * (D / 2) + tig * (D / 8), wa);
-                lds_words(blk[u] + (r + 8) * (D / 2) + tig * (D / 8), wb);
-                float dot[NT][G][4];
+                lds_words(smem + k_at + u * U, wa[u]);
+                lds_words(smem + k_at + u * U + 8 * (D / 2), wb[u]);
+            }
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+            for (int w = 0; w < 2 * G; ++w) {
 #pragma unroll
-                    for (int g = 0; g < G; ++g)
+                for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) dot[n][g][k] = 0.f;
-#pragma unroll
-                for (int w = 0; w < 2 * G; ++w) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const uint32_t x = wa[w] >> (8 * half), y = wb[w] >> (8 * half);
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t x = wa[u][w] >> (8 * half), y = wb[u][w] >> (8 * half);
                         const uint32_t a0 = x & 0x000f000fu, a1 = y & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = y & 0x00f000f0u;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) mma_16816(dot[n][w % G], a0, a1, a2, a3, q[n][w][2 * half], q[n][w][2 * half + 1]);
+                        for (int n = 0; n < NT; ++n) {
+                            if (w < G && half == 0) mma_16816_from_zero(dot[u][n][w % G], a0, a1, a2, a3, q[n][w][0], q[n][w][1]);
+                            else mma_16816(dot[u][n][w % G], a0, a1, a2, a3, q[n][w][2 * half], q[n][w][2 * half + 1]);
+                        }
                     }
                 }
+            }
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+            for (int u = 0; u < NU; ++u) {
+#pragma unroll
+                for (int e = 0; e < NE; ++e) {
                     uint32_t kp[G];
-                    const uint32_t pairs = blk[u] + page * D + (r + 8 * e) * (G * 4);
-                    lds_words(pairs, kp);
-                    lds_words(pairs + page * (G * 4), vp[u][e]);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) sc[u][e][n] = pack2(0.f, 0.f);
+                    lds_words(smem + pair_at + u * U_PAIRS + 8 * e * (G * 4), kp);
+                    lds_words(smem + pair_at + u * U_PAIRS + 8 * e * (G * 4) + PAIRS, vp[u][e]);
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
                         const float2 sz = pair_of(kp[g]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            const f32x2 t = fma2(pack2(dot[n][g][2 * e], dot[n][g][2 * e + 1]), to_log2[n], q8[n][g]);
-                            sc[u][e][n] = fma2(pack2(sz.x, sz.x), t, sc[u][e][n]);
-                            sc[u][e][n] = fma2(pack2(sz.y, sz.y), qz[n][g], sc[u][e][n]);
+                            f32x2 c = pack2(dot[u][n][g][2 * e], dot[u][n][g][2 * e + 1]);
+                            if constexpr (W >= 2) {          // this lane's octet
+                                if (my_e) c = pack2(dot[u][n][g][2], dot[u][n][g][3]);
+                            }
+                            if constexpr (W == 4) {
+                                if (my_u) c = my_e ? pack2(dot[1][n][g][2], dot[1][n][g][3]) : pack2(dot[1][n][g][0], dot[1][n][g][1]);
+                            }
+                            const f32x2 t = fma2(c, to_log2[n], q8[n][g]);
+                            // one factor for two heads: two instructions, where the packed form needs two moves for the pair
+                            const float x = g == 0 ? sz.y * qz[n][g].x : fmaf(sz.y, qz[n][g].x, sc[u][e][n].x);
+                            const float y = g == 0 ? sz.y * qz[n][g].y : fmaf(sz.y, qz[n][g].y, sc[u][e][n].y);
+                            sc[u][e][n] = pack2(fmaf(sz.x, t.x, x), fmaf(sz.x, t.y, y));
                         }
-                    }
-                    if (u * 16 + 8 * e + row >= left) {      // no such position: whatever the page holds there
-#pragma unroll
-                        for (int n = 0; n < NT; ++n) sc[u][e][n] = pack2(-INFINITY, -INFINITY);
-#pragma unroll
-                        for (int g = 0; g < G; ++g) vp[u][e][g] = 0u;
                     }
                 }
             }
-            // ---- reference maximum: moved only when a score runs ahead of it ----
-            bool ahead = false;
-            f32x2 mx[NT];
+            if (left < 32) {                                 // positions that do not exist: whatever the page holds there
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mx[n].x = fmaxf(fmaxf(sc[0][0][n].x, sc[0][1][n].x), fmaxf(sc[1][0][n].x, sc[1][1][n].x));
-                mx[n].y = fmaxf(fmaxf(sc[0][0][n].y, sc[0][1][n].y), fmaxf(sc[1][0][n].y, sc[1][1][n].y));
-                ahead |= mx[n].x > m_ref[n].x + kLazy || mx[n].y > m_ref[n].y + kLazy;
+                for (int u = 0; u < NU; ++u)
+#pragma unroll
+                    for (int e = 0; e < NE; ++e)
+                        if ((u + my_u) * 16 + 8 * (e + my_e) + row >= left) {
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) sc[u][e][n] = pack2(-INFINITY, -INFINITY);
+#pragma unroll
+                            for (int g = 0; g < G; ++g) vp[u][e][g] = 0u;
+                        }
             }
-            if (__any_sync(0xffffffffu, ahead)) {
+            // ---- reference: moved only when a product would run ahead of it ----
+            __half2 big = *reinterpret_cast<const __half2*>(&vp[0][0][0]);       // largest value scale, in the low half
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) big = __hmax2(big, *reinterpret_cast<const __half2*>(&vp[u][e][g]));
+            const float big_scale = __low2float(big);
+            float over = -INFINITY;                          // the largest score above its reference
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+                for (int e = 0; e < NE; ++e)
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const f32x2 x = add2(sc[u][e][n], neg[n]);
+                        over = max3(over, x.x, x.y);
+                    }
+            if (__any_sync(0xffffffffu, over > room || big_scale > top)) {
+                const uint32_t top_bits = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(big_scale, top)));
+                const int exponent = (int)((top_bits + 0x7fffffu) >> 23);                        // rounded up
+                top = __int_as_float(exponent << 23);
+                room = kTop + kSlack + 127.0f - (float)exponent;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
+                    f32x2 mx = sc[0][0][n];
+#pragma unroll
+                    for (int u = 0; u < NU; ++u)
+#pragma unroll
+                        for (int e = 0; e < NE; ++e) mx = pack2(fmaxf(mx.x, sc[u][e][n].x), fmaxf(mx.y, sc[u][e][n].y));
 #pragma unroll
                     for (int o = 4; o < 32; o <<= 1) {
-                        mx[n].x = fmaxf(mx[n].x, __shfl_xor_sync(0xffffffffu, mx[n].x, o));
-                        mx[n].y = fmaxf(mx[n].y, __shfl_xor_sync(0xffffffffu, mx[n].y, o));
+                        mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
+                        mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
                     }
-                    const float nx = fmaxf(m_ref[n].x, mx[n].x), ny = fmaxf(m_ref[n].y, mx[n].y);
-                    const float cx = m_ref[n].x == nx ? 1.f : ex2_approx(m_ref[n].x - nx), cy = m_ref[n].y == ny ? 1.f : ex2_approx(m_ref[n].y - ny);
-                    m_ref[n] = pack2(nx, ny);
-                    l2[n] = mul2(l2[n], pack2(cx, cy));
+                    // the reference goes up to kTop - (largest scale) below the largest score, never down
+                    const f32x2 to = pack2(fminf(neg[n].x, room - kSlack - mx.x), fminf(neg[n].y, room - kSlack - mx.y));
+                    const f32x2 keep = pack2(ex2_approx(to.x - neg[n].x), ex2_approx(to.y - neg[n].y));
+                    neg[n] = to;
+                    l2[n] = mul2(l2[n], keep);
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
-                        w2[n][g] = mul2(w2[n][g], pack2(cx, cy));
-                        ones[n][g][0] *= cx, ones[n][g][1] *= cy;
+                        w2[n][g] = mul2(w2[n][g], keep);
+                        ones[n][g][0] *= keep.x, ones[n][g][1] *= keep.y;
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) acc[n][g][t][0] *= cx, acc[n][g][t][1] *= cy, acc[n][g][t][2] *= cx, acc[n][g][t][3] *= cy;
+                        for (int t = 0; t < 4; ++t) acc[n][g][t][0] *= keep.x, acc[n][g][t][1] *= keep.y, acc[n][g][t][2] *= keep.x, acc[n][g][t][3] *= keep.y;
                     }
                 }
             }
             // ---- probabilities, and the second product ----
-            f32x2 neg[NT];                                   // a row without a finite score yet: every p is 2^-inf
+            uint32_t turned[NU][NE][NT][G];                  // P with columns as rows
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
-                neg[n] = pack2(m_ref[n].x == -INFINITY ? 0.f : -m_ref[n].x, m_ref[n].y == -INFINITY ? 0.f : -m_ref[n].y);
+            for (int u = 0; u < NU; ++u) {
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                if (u == 1 && left <= 16) break;
-                uint32_t pb[NT][G][2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < NE; ++e) {
                     f32x2 p[NT];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
@@ -424,20 +515,30 @@ kv4_scan_kernel(const Kv4Args a) {
                         const float2 sz = pair_of(vp[u][e][g]);
 #pragma unroll
                         for (int n = 0; n < NT; ++n) {
-                            w2[n][g] = fma2(p[n], pack2(sz.y, sz.y), w2[n][g]);
-                            const f32x2 ps = mul2(p[n], pack2(sz.x, sz.x));
-                            pb[n][g][e] = transpose8x8(pack_half2(ps.x, ps.y));
+                            w2[n][g] = pack2(fmaf(p[n].x, sz.y, w2[n][g].x), fmaf(p[n].y, sz.y, w2[n][g].y));
+                            turned[u][e][n][g] = transpose8x8(pack_half2(p[n].x * sz.x, p[n].y * sz.x));
                         }
                     }
                 }
-                const int r = ((warp * 32 + u * 16) & (page - 1)) + vrow;
-                const uint32_t vaddr = blk[u] + page * (D / 2) + r * (D / 2) + gid * (G * 4);
-                const int next = ((vrow ^ 1) - vrow) * (D / 2);      // the odd position of the pair
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                uint32_t pb[NT][G][2];                       // an octet's P, in the columns of the copy that has it
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            if constexpr (W == 1) pb[n][g][e] = turned[u][e][n][g];
+                            else pb[n][g][e] = copy == (W == 2 ? e : 2 * u + e) ? turned[W == 4 ? 0 : u][0][n][g] : 0u;
+                        }
                 uint32_t v0[G], v1[G], v2[G], v3[G];
-                lds_words(vaddr, v0);
-                lds_words(vaddr + next, v1);
-                lds_words(vaddr + 8 * (D / 2), v2);
-                lds_words(vaddr + 8 * (D / 2) + next, v3);
+                // the odd position of the pair: blocks and stages are multiples of two rows
+                lds_words(smem + v_at + u * U, v0);
+                lds_words(smem + (v_at ^ (D / 2)) + u * U, v1);
+                lds_words(smem + v_at + u * U + 8 * (D / 2), v2);
+                lds_words(smem + (v_at ^ (D / 2)) + u * U + 8 * (D / 2), v3);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
 #pragma unroll
@@ -459,15 +560,21 @@ kv4_scan_kernel(const Kv4Args a) {
                 }
             }
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(empty(s));
-
-        const bool row_ends = cur.tile + 1 == cur.tiles, seg_ends = row_ends || i + 1 == run;
-        if (seg_ends) {
-            // ---- the four warps' rows become one ----
-            float* mine_rows = merge + warp * (Cfg::HEADS * ROW);
+            if (k + 1 < pieces) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(empty(s));
+                next_stage();
+            }
+        }
+        {
+            // ---- the rows of the four warps and of the copies become one, in the stage that all have read ----
+            float* merge = reinterpret_cast<float*>(smem + s * Cfg::TILE_BYTES);
+            const bool whole = seg_first == 0 && row_ends;
+            float* part = a.parts + ((long long)blockIdx.x * 2 + (seg_first == 0 ? 1 : 0)) * a.group * ROW;
+            __half* out = a.out + ((long long)cur.b * heads + (long long)cur.h * a.group) * D;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
+                __syncthreads();
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) {
                     l2[n].x += __shfl_xor_sync(0xffffffffu, l2[n].x, o), l2[n].y += __shfl_xor_sync(0xffffffffu, l2[n].y, o);
@@ -475,7 +582,7 @@ kv4_scan_kernel(const Kv4Args a) {
                     for (int g = 0; g < G; ++g)
                         w2[n][g].x += __shfl_xor_sync(0xffffffffu, w2[n][g].x, o), w2[n][g].y += __shfl_xor_sync(0xffffffffu, w2[n][g].y, o);
                 }
-                float* r0 = mine_rows + (n * 8 + 2 * tig) * ROW;     // heads 2 tig, 2 tig + 1
+                float* r0 = merge + (warp * 8 + 2 * tig) * ROW;      // columns 2 tig, 2 tig + 1
                 float* r1 = r0 + ROW;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
@@ -488,50 +595,49 @@ kv4_scan_kernel(const Kv4Args a) {
                     }
                 }
                 if (gid == 0) {
-                    r0[D] = m_ref[n].x, r0[D + 1] = l2[n].x;
-                    r1[D] = m_ref[n].y, r1[D + 1] = l2[n].y;
+                    r0[D] = -neg[n].x, r0[D + 1] = l2[n].x;
+                    r1[D] = -neg[n].y, r1[D + 1] = l2[n].y;
                 }
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            const bool whole = seg_first == 0 && row_ends;
-            float* part = a.parts + ((long long)blockIdx.x * 2 + (seg_first == 0 ? 1 : 0)) * a.group * ROW;
-            __half* out = a.out + ((long long)cur.b * heads + (long long)cur.h * a.group) * D;
-            for (int e = threadIdx.x; e < a.group * (D / 4); e += kWarps * 32) {
-                const int j = e / (D / 4), d = (e - j * (D / 4)) * 4;
-                const float* r = merge + j * ROW;
-                float m = -INFINITY;
+                __syncthreads();
+                const int real = min(a.group - n * 8, HEADS);
+                for (int e = threadIdx.x; e < real * (D / 4); e += kScanThreads) {
+                    const int c = e / (D / 4), d = (e - c * (D / 4)) * 4, j = n * 8 + c;
+                    const float* r = merge + c * ROW;        // row (warp, copy) of the head: 8 warp + HEADS copy further
+                    float m = r[D];
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) m = fmaxf(m, r[w * (Cfg::HEADS * ROW) + D]);
-                float l = 0.f;
-                float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+                    for (int w = 1; w < kWarps * W; ++w) m = fmaxf(m, r[w * HEADS * ROW + D]);
+                    float l = 0.f;
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float* rw = r + w * (Cfg::HEADS * ROW);
-                    const float f = rw[D] == -INFINITY && rw[D + 1] == 0.f ? 0.f : ex2_approx(rw[D] - (m == -INFINITY ? 0.f : m));
-                    // a row whose scores were all NaN has no maximum but its sum is NaN: it stays in
-                    const float keep = rw[D + 1] != rw[D + 1] ? 1.f : f;
-                    const float4 x = *reinterpret_cast<const float4*>(rw + d);
-                    l = fmaf(keep, rw[D + 1], l);
-                    o.x = fmaf(keep, x.x, o.x), o.y = fmaf(keep, x.y, o.y), o.z = fmaf(keep, x.z, o.z), o.w = fmaf(keep, x.w, o.w);
-                }
-                if (whole) {
-                    const float inv = 1.0f / l;
-                    *reinterpret_cast<uint2*>(out + (long long)j * D + d) = make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
-                } else {
-                    *reinterpret_cast<float4*>(part + j * ROW + d) = o;
-                    if (d == 0) part[j * ROW + D] = m, part[j * ROW + D + 1] = l;
+                    for (int w = 0; w < kWarps * W; ++w) {
+                        const float* rw = r + w * HEADS * ROW;
+                        const float f = ex2_approx(rw[D] - m);       // (a row of NaN sums stays NaN under any factor)
+                        const float4 x = *reinterpret_cast<const float4*>(rw + d);
+                        l = fmaf(f, rw[D + 1], l);
+                        o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
+                    }
+                    if (whole) {
+                        const float inv = 1.0f / l;
+                        *reinterpret_cast<uint2*>(out + (long long)j * D + d) = make_uint2(pack_half2(o.x * inv, o.y * inv), pack_half2(o.z * inv, o.w * inv));
+                    } else {
+                        *reinterpret_cast<float4*>(part + j * ROW + d) = o;
+                        if (d == 0) part[j * ROW + D] = m, part[j * ROW + D + 1] = l;
+                    }
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (i + 1 < run) {
-                advance(a, cur);
-                seg_first = cur.tile;
-                begin_row();
-            }
-        } else {
-            ++cur.tile;
+            fence_proxy_async();                                 // before the next copy into this stage
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(empty(s));
+        next_stage();
+        if (more) next_row(a, cur);
+        tile = 0;
     }
+    return;
+late:                                        // a wait gave up: copies still in flight land before this warp leaves
+    if (lane == 0) note(a, kNotedTimeout, 1u);
+    for (int k = 0; k < Cfg::STAGES; ++k)
+        for (uint32_t ph = 0; ph < 2; ++ph) mbar_wait_bounded(full(k), ph, 64u);
 }
 
 // One CTA per (request, key head) row and query head: adds up the partial rows the scan left for it, if it left any;
@@ -565,14 +671,13 @@ kv4_merge_kernel(const Kv4Args a, int nctas) {
     const int parts = c1 - c0 + 1;
     // the first CTA left its piece in slot 1 (the row began there), the others in slot 0
     auto part_of = [&](int i) { return a.parts + ((long long)((c0 + i) * 2 + (i == 0 ? 1 : 0)) * a.group + j) * ROW; };
-    float m = -INFINITY;
+    float m = -kNoReference;
     for (int i = threadIdx.x; i < parts; i += 128) m = fmaxf(m, part_of(i)[D]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     if ((threadIdx.x & 31) == 0) s_m[threadIdx.x >> 5] = m;
     __syncthreads();
     m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    const float ref = m == -INFINITY ? 0.f : m;
     const int k = threadIdx.x / LPR, d = (threadIdx.x % LPR) * 4;
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -581,7 +686,7 @@ kv4_merge_kernel(const Kv4Args a, int nctas) {
         const float* p = part_of(i);
         const float4 x = *reinterpret_cast<const float4*>(p + d);
         const float2 ml = *reinterpret_cast<const float2*>(p + D);
-        const float f = ml.y != ml.y ? 1.f : ex2_approx(ml.x - ref);
+        const float f = ex2_approx(ml.x - m);
         l = fmaf(f, ml.y, l);
         o.x = fmaf(f, x.x, o.x), o.y = fmaf(f, x.y, o.y), o.z = fmaf(f, x.z, o.z), o.w = fmaf(f, x.w, o.w);
     }
@@ -612,12 +717,14 @@ struct Kv4Layout {
     size_t prefix_off, noted_off, parts_off, total;
 };
 
-int blocks_of_8(int group) { return group <= 8 ? 1 : 2; }
+int resident_ctas(int group) {
+    return group <= 2 ? Kv4Cfg<128, 1, 4>::CTAS : group <= 4 ? Kv4Cfg<128, 1, 2>::CTAS : group <= 8 ? Kv4Cfg<128, 1, 1>::CTAS : Kv4Cfg<128, 2, 1>::CTAS;
+}
 
 Kv4Layout kv4_layout(int B, int kv_heads, int group, int max_len, int D) {
     Kv4Layout y;
     const long long tiles = (long long)B * kv_heads * ((max_len + kTile - 1) / kTile);
-    const long long resident = (long long)sms() * (blocks_of_8(group) == 1 ? Kv4Cfg<128, 1>::CTAS : Kv4Cfg<128, 2>::CTAS);
+    const long long resident = (long long)sms() * resident_ctas(group);
     y.ctas = (int)(tiles < resident ? tiles : resident);
     y.prefix_off = 256;
     y.noted_off = y.prefix_off + round_up((size_t)(B + 1) * 4, 256);
@@ -631,19 +738,37 @@ bool kv4_shape_ok(int B, int heads, int kv_heads, int max_len, int D) {
            (long long)B * kv_heads * ((max_len + kTile - 1) / kTile) < (1ll << 31) && (long long)B * kv_heads < (1ll << 31);
 }
 
-template <int D, int NT>
+template <int D, int NT, int W, int PAGE>
 int launch_kv4(const Kv4Args& a, int ctas, cudaStream_t st) {
-    using Cfg = Kv4Cfg<D, NT>;
+    using Cfg = Kv4Cfg<D, NT, W>;
     static bool attr_done[64] = {false};
     int dev = 0;
     I8TK_CUDA(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        I8TK_CUDA(cudaFuncSetAttribute(kv4_scan_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+        I8TK_CUDA(cudaFuncSetAttribute(kv4_scan_kernel<D, NT, W, PAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM));
+        // the merge under the same split of L1 and shared memory: an SM changes it only when it is empty, and then the
+        // two kernels do not overlap
+        I8TK_CUDA(cudaFuncSetAttribute(kv4_scan_kernel<D, NT, W, PAGE>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
+        I8TK_CUDA(cudaFuncSetAttribute(kv4_merge_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, 100));
         if (dev >= 0 && dev < 64) attr_done[dev] = true;
     }
-    I8TK_CUDA(launch_after(kv4_scan_kernel<D, NT>, dim3((unsigned)ctas), dim3(kScanThreads), Cfg::SMEM, st, a));
+    I8TK_CUDA(launch_after(kv4_scan_kernel<D, NT, W, PAGE>, dim3((unsigned)ctas), dim3(kScanThreads), Cfg::SMEM, st, a));
     I8TK_CUDA(launch_after(kv4_merge_kernel<D>, dim3((unsigned)(a.B * a.kv_heads), (unsigned)a.group), dim3(128), 0, st, a, ctas));
     return I8TK_OK;
+}
+template <int D, int NT, int W>
+int launch_page(const Kv4Args& a, int page, int ctas, cudaStream_t st) {
+    if (page == 16) return launch_kv4<D, NT, W, 16>(a, ctas, st);
+    if (page == 32) return launch_kv4<D, NT, W, 32>(a, ctas, st);
+    if (page == 64) return launch_kv4<D, NT, W, 64>(a, ctas, st);
+    return launch_kv4<D, NT, W, 128>(a, ctas, st);
+}
+template <int D>
+int launch_group(const Kv4Args& a, int page, int ctas, cudaStream_t st) {
+    if (a.group <= 2) return launch_page<D, 1, 4>(a, page, ctas, st);
+    if (a.group <= 4) return launch_page<D, 1, 2>(a, page, ctas, st);
+    if (a.group <= 8) return launch_page<D, 1, 1>(a, page, ctas, st);
+    return launch_page<D, 2, 1>(a, page, ctas, st);
 }
 
 }  // namespace
@@ -680,14 +805,10 @@ extern "C" int i8tk_decode_attention_kv4(const int8_t* Q, int64_t q_stride, cons
                  "decode workspace too small: need %zu bytes, got %zu", y.total, workspace_bytes);
     I8TK_REQUIRE(aligned_to(workspace, 256), I8TK_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
     unsigned char* ws = static_cast<unsigned char*>(workspace);
-    int shift = 4;
-    while ((1 << shift) < page_size) ++shift;
     const Kv4Args a{Q, sQ, q_stride, sq_stride, static_cast<const unsigned char*>(pool), page_table, seq_lens,
-                    static_cast<__half*>(out_f16), batch, kv_heads, group, max_seq_len, shift, max_pages_per_seq, (int)num_pages,
+                    static_cast<__half*>(out_f16), batch, kv_heads, group, max_seq_len, max_pages_per_seq, (int)num_pages,
                     1.4426950408889634f / sqrtf((float)head_dim), reinterpret_cast<uint32_t*>(ws),
                     reinterpret_cast<int*>(ws + y.prefix_off), reinterpret_cast<uint32_t*>(ws + y.noted_off), reinterpret_cast<float*>(ws + y.parts_off)};
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (blocks_of_8(group) == 1)
-        return head_dim == 64 ? launch_kv4<64, 1>(a, y.ctas, st) : launch_kv4<128, 1>(a, y.ctas, st);
-    return head_dim == 64 ? launch_kv4<64, 2>(a, y.ctas, st) : launch_kv4<128, 2>(a, y.ctas, st);
+    return head_dim == 64 ? launch_group<64>(a, page_size, y.ctas, st) : launch_group<128>(a, page_size, y.ctas, st);
 }

@@ -8,10 +8,15 @@
 //
 // All in fp32 from the 16-bit input, one rounding at the end (to the input's type, or to the code).
 //
-// Bound by memory: 2 bytes read and 2 (or 1) written per channel.  A row is held by D/8 lanes, eight channels
-// (one 16-byte load) each, so the norm and the row maximum are shuffles and the partner of a half-split rotation is
-// one shuffle away.  A warp works on kRows rows per lane group of ONE token: their loads are in flight together, and
-// the eight cosines and sines a lane needs (64 bytes, four times the data of a row) are read once for all of them.
+// Memory moves 2 bytes in and 2 (or 1) out per channel; at that rate an SM has about 15 instruction slots of a lane
+// per channel, so the arithmetic is what has to be kept short:
+// * norm, weight and rotation are u = x * (w c) + z * (w' s) and y = r u, where z is the partner channel and w' its
+//   weight.  The products with the weights are made once for the rows of a warp, which are heads of one kind (query,
+//   key or value) of ONE token; the partner comes by one shuffle of the raw 16-bit pair (half split) or by swapping
+//   the halves of a word (interleaved).  Packed fp32 pairs throughout.
+// * r never touches the channels in the quantised form: it goes into the scale.
+// * Rounding is the addition of 1.5 * 2^23, the code is the low byte of the sum.
+// A row is held by D/8 lanes, eight channels (one 16-byte load) each; a warp has kRows rows per lane group in flight.
 #include "common.cuh"
 
 #include <cuda_bf16.h>
@@ -35,7 +40,7 @@ struct QkArgs {
     float eps;
     long long tokens;
     int heads, kv_heads;
-    int units;                    // warps per token
+    int q_units, k_units, units;  // warps per token: of query heads, of key heads, in all
     void* out;                    // [tokens][heads + kv_heads][D] in the input's type (float form), or
     int8_t* codes;                // [tokens][heads + 2 kv_heads][D]
     float* scales;                // [tokens][heads + 2 kv_heads]
@@ -55,13 +60,16 @@ __device__ __forceinline__ uint32_t narrow(const __nv_bfloat16*, float a, float 
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// round half to even of y / s as the quantiser defines it: the product with the rounded reciprocal is within a few
-// ulps of the quotient, so only quotients next to a tie need the division itself
-__device__ __forceinline__ int code_of(float y, float s, float inv) {
-    const float t = y * inv;
-    float r = rintf(t);
-    if (fabsf(t - r) > 0.4999f) r = rintf(__fdiv_rn(y, s));
-    return (int)r;
+// x / 127 correctly rounded: a quotient from the rounded reciprocal, corrected by its exact remainder (Markstein)
+__device__ __forceinline__ float div127(float x) {
+    const float r = 1.0f / 127.0f;
+    const float q = x * r;
+    return fmaf(fmaf(-127.0f, q, x), r, q);
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 template <typename T, int D, bool QUANT>
@@ -69,132 +77,163 @@ __global__ void __launch_bounds__(kThreads)
 qk_norm_rope_kernel(const QkArgs a) {
     constexpr int LPR = D / 8;                       // lanes per row
     constexpr int GROUPS = 32 / LPR;                 // rows a warp holds side by side
+    constexpr int PER = kRows * GROUPS;              // rows of a warp
+    const T* tag = nullptr;
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const long long unit = (long long)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
-    const long long t = unit / a.units;
+    const int lane = threadIdx.x & 31, sub = lane % LPR, d0 = sub * 8;
+    const unsigned chunk = blockIdx.x / (unsigned)a.units;
+    const int unit = (int)(blockIdx.x - chunk * (unsigned)a.units);
+    const long long t = (long long)chunk * (kThreads / 32) + (threadIdx.x >> 5);
     if (t >= a.tokens) return;                       // whole warps leave
-    const int first = (int)(unit - t * a.units) * (kRows * GROUPS) + lane / LPR;   // this group's first head
-    const int sub = lane % LPR;
-    const int d0 = sub * 8;
-    const int rotated = a.heads + a.kv_heads;        // heads that are normed and rotated; the rest are values
-    const int total = QUANT ? rotated + a.kv_heads : rotated;
+    // units of query heads first, then of key heads, then of value heads
+    const int kind = unit < a.q_units ? 0 : unit < a.q_units + a.k_units ? 1 : 2;
+    const int head0 = kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads;
+    const int count = kind == 0 ? a.heads : a.kv_heads;
+    const int first = (unit - (kind == 0 ? 0 : kind == 1 ? a.q_units : a.q_units + a.k_units)) * PER + lane / LPR;
+    const int total = a.heads + a.kv_heads * (QUANT ? 2 : 1);
 
-    const T* row = static_cast<const T*>(a.qkv) + t * a.row_stride + d0;
+    const T* row = static_cast<const T*>(a.qkv) + t * a.row_stride + (long long)head0 * D + d0;
     uint4 raw[kRows];
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const int h = first + i * GROUPS;
-        raw[i] = h < total ? *reinterpret_cast<const uint4*>(row + (long long)h * D) : make_uint4(0u, 0u, 0u, 0u);
+        raw[i] = h < count ? *reinterpret_cast<const uint4*>(row + (long long)h * D) : make_uint4(0u, 0u, 0u, 0u);
     }
-    float c[8], s[8];
-    const bool turn = a.positions != nullptr;
+
+    // ---- what the rows share: w c and w' s of this lane's channels ----
+    f32x2 wc[4], ws[4];
     const int half_r = a.R >> 1;
-    const bool mine = turn && d0 < a.R;              // R is a multiple of 16: a lane's channels are all in or all out
-    if (mine) {
-        const int pos = a.positions[t];
-        const bool known = pos >= 0 && pos < a.rope_rows;
-        if (a.interleaved) {                         // four pairs of this lane
-            const float* tab = a.rope + (long long)(known ? pos : 0) * a.R + (d0 >> 1);
-            const float4 cc = *reinterpret_cast<const float4*>(tab), ss = *reinterpret_cast<const float4*>(tab + half_r);
-            c[0] = cc.x, c[1] = cc.y, c[2] = cc.z, c[3] = cc.w;
-            s[0] = ss.x, s[1] = ss.y, s[2] = ss.z, s[3] = ss.w;
-        } else {
-            const float* tab = a.rope + (long long)(known ? pos : 0) * a.R + (d0 < half_r ? d0 : d0 - half_r);
-            const float sign = d0 < half_r ? -1.0f : 1.0f;
+    const bool norm = kind < 2 && a.q_weight != nullptr;
+    const bool turn = kind < 2 && a.positions != nullptr && d0 < a.R;   // R is a multiple of 16: all of a lane's channels or none
+    const int partner = d0 < half_r ? sub + half_r / 8 : sub - half_r / 8;     // lane of the half-split partner
+    const int from = lane - sub + (turn && !a.interleaved ? partner : sub);
+    bool known = true;                               // a position without a table row shows in the result
+    if (kind < 2) {
+        const float* weight = kind == 0 ? a.q_weight : a.k_weight;
+        float w[8], wp[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) w[k] = wp[k] = 1.0f;
+        if (norm) {
+            const float* at = weight + d0;
+            const float* other = weight + (turn && !a.interleaved ? partner * 8 : d0);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float4 cc = *reinterpret_cast<const float4*>(tab + 4 * k), ss = *reinterpret_cast<const float4*>(tab + half_r + 4 * k);
-                c[4 * k] = cc.x, c[4 * k + 1] = cc.y, c[4 * k + 2] = cc.z, c[4 * k + 3] = cc.w;
-                s[4 * k] = sign * ss.x, s[4 * k + 1] = sign * ss.y, s[4 * k + 2] = sign * ss.z, s[4 * k + 3] = sign * ss.w;
+                const float4 x = *reinterpret_cast<const float4*>(at + 4 * k), y = *reinterpret_cast<const float4*>(other + 4 * k);
+                w[4 * k] = x.x, w[4 * k + 1] = x.y, w[4 * k + 2] = x.z, w[4 * k + 3] = x.w;
+                wp[4 * k] = y.x, wp[4 * k + 1] = y.y, wp[4 * k + 2] = y.z, wp[4 * k + 3] = y.w;
             }
         }
-        if (!known) {                                // a position without a table row shows in the result
 #pragma unroll
-            for (int k = 0; k < 8; ++k) c[k] = s[k] = __int_as_float(0x7fc00000);
+        for (int k = 0; k < 4; ++k) wc[k] = pack2(w[2 * k], w[2 * k + 1]), ws[k] = pack2(0.f, 0.f);
+        if (a.positions != nullptr) {
+            const int pos = a.positions[t];
+            known = pos >= 0 && pos < a.rope_rows;
+            const float* tab = a.rope + (long long)(known ? pos : 0) * a.R;
+            if (turn && a.interleaved) {             // four pairs of this lane: the partner is the other half of a word
+                const float4 c = *reinterpret_cast<const float4*>(tab + (d0 >> 1)), s = *reinterpret_cast<const float4*>(tab + half_r + (d0 >> 1));
+                const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    wc[k] = pack2(w[2 * k] * cs[k], w[2 * k + 1] * cs[k]);
+                    ws[k] = pack2(-w[2 * k + 1] * sn[k], w[2 * k] * sn[k]);
+                }
+            } else if (turn) {
+                const float* c0 = tab + (d0 < half_r ? d0 : d0 - half_r);
+                const float sign = d0 < half_r ? -1.0f : 1.0f;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const float4 c = *reinterpret_cast<const float4*>(c0 + 4 * k), s = *reinterpret_cast<const float4*>(c0 + half_r + 4 * k);
+                    wc[2 * k] = pack2(w[4 * k] * c.x, w[4 * k + 1] * c.y), wc[2 * k + 1] = pack2(w[4 * k + 2] * c.z, w[4 * k + 3] * c.w);
+                    ws[2 * k] = pack2(wp[4 * k] * (sign * s.x), wp[4 * k + 1] * (sign * s.y));
+                    ws[2 * k + 1] = pack2(wp[4 * k + 2] * (sign * s.z), wp[4 * k + 3] * (sign * s.w));
+                }
+            }
+            if (turn && !known) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) wc[k] = pack2(__int_as_float(0x7fc00000), __int_as_float(0x7fc00000));
+            }
         }
     }
-    // the partner lane of a half-split rotation
-    const int partner = lane - sub + (d0 < half_r ? sub + half_r / 8 : sub - half_r / 8);
-    const int from = mine ? partner : lane;
 
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
         const int h = first + i * GROUPS;
-        const uint32_t w4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
-        float y[8];
+        if (h - lane / LPR >= count) break;          // the whole warp is past the last head
+        const uint32_t x4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        f32x2 u[4];
+        float r = 1.0f;
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const float2 v = widen(static_cast<const T*>(nullptr), w4[k]);
-            y[2 * k] = v.x, y[2 * k + 1] = v.y;
+        for (int k = 0; k < 4; ++k) u[k] = widen(tag, x4[k]);
+        if (norm) {
+            f32x2 sq = mul2(u[0], u[0]);
+#pragma unroll
+            for (int k = 1; k < 4; ++k) sq = fma2(u[k], u[k], sq);
+            float ss = sq.x + sq.y;
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            r = rsqrtf(ss * (1.0f / D) + a.eps);
         }
-        const bool is_qk = h < rotated;
-        const float* weight = h < a.heads ? a.q_weight : a.k_weight;
-        float ss = 0.f;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) ss = fmaf(y[k], y[k], ss);
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (is_qk && weight != nullptr) {
-            const float r = rsqrtf(ss * (1.0f / D) + a.eps);
-            const float4 wa = *reinterpret_cast<const float4*>(weight + d0), wb = *reinterpret_cast<const float4*>(weight + d0 + 4);
-            y[0] *= r * wa.x, y[1] *= r * wa.y, y[2] *= r * wa.z, y[3] *= r * wa.w;
-            y[4] *= r * wb.x, y[5] *= r * wb.y, y[6] *= r * wb.z, y[7] *= r * wb.w;
-        }
-        if (turn) {
+        if (kind < 2) {
+            uint32_t z4[4];
             if (a.interleaved) {
-                if (mine && is_qk) {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float u = y[2 * k], v = y[2 * k + 1];
-                        y[2 * k] = u * c[k] - v * s[k];
-                        y[2 * k + 1] = v * c[k] + u * s[k];
-                    }
-                }
+                for (int k = 0; k < 4; ++k) z4[k] = prmt(x4[k], 0u, 0x1032u);
             } else {
-                float z[8];
 #pragma unroll
-                for (int k = 0; k < 8; ++k) z[k] = __shfl_sync(0xffffffffu, y[k], from);
-                if (mine && is_qk) {
+                for (int k = 0; k < 4; ++k) z4[k] = __shfl_sync(0xffffffffu, x4[k], from);
+            }
 #pragma unroll
-                    for (int k = 0; k < 8; ++k) y[k] = y[k] * c[k] + z[k] * s[k];
-                }
+            for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], wc[k]);
+            if (turn) {                              // (a lane outside the rotated channels must not see 0 * infinity)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) u[k] = fma2(widen(tag, z4[k]), ws[k], u[k]);
             }
         }
         if constexpr (!QUANT) {
-            if (h < total) {
-                const T* tag = nullptr;
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (t * total + h) * D + d0) =
-                    make_uint4(narrow(tag, y[0], y[1]), narrow(tag, y[2], y[3]), narrow(tag, y[4], y[5]), narrow(tag, y[6], y[7]));
-            }
-        } else {
-            float mx = 0.f;
+            const f32x2 r2 = pack2(r, r);
 #pragma unroll
-            for (int k = 0; k < 8; ++k) mx = fmaxf(mx, fabsf(y[k]));
+            for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], r2);
+            if (h < count)
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (t * total + head0 + h) * D + d0) =
+                    make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
+        } else {
+            float mx = max3(max3(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y), max3(fabsf(u[2].x), fabsf(u[2].y), fmaxf(fabsf(u[3].x), fabsf(u[3].y))));
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            // a row whose position has no table entry is NaN throughout its rotated part: its scale says so
-            float scale = __fdiv_rn(fmaxf(mx, 1e-8f), 127.0f);
-            const bool bad = mine && is_qk && c[0] != c[0];
-            if (__any_sync(0xffffffffu, bad)) {
-                const unsigned who = __ballot_sync(0xffffffffu, bad);
-                const unsigned group = (LPR == 32 ? 0xffffffffu : ((1u << LPR) - 1u) << (lane - sub));
-                if (who & group) scale = __int_as_float(0x7fc00000);
-            }
-            const float inv = __frcp_rn(scale);
-            int q[8];
+            const float scale = known ? div127(fmaxf(mx * r, 1e-8f)) : __int_as_float(0x7fc00000);
+            const float inv = rcp_approx(scale) * r;
+            const f32x2 inv2 = pack2(inv, inv), magic = pack2(12582912.f, 12582912.f);
+            f32x2 q[4];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) q[k] = code_of(y[k], scale, inv);
-            if (h < total) {
-                const uint32_t lo = prmt(prmt(q[0], q[1], 0x0040), prmt(q[2], q[3], 0x0040), 0x5410);
-                const uint32_t hi = prmt(prmt(q[4], q[5], 0x0040), prmt(q[6], q[7], 0x0040), 0x5410);
-                *reinterpret_cast<uint2*>(a.codes + (t * total + h) * D + d0) = make_uint2(lo, hi);
-                if (sub == 0) a.scales[t * total + h] = scale;
-                if (a.k_out != nullptr && h >= a.heads && is_qk) {
-                    const T* tag = nullptr;
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (t * a.kv_heads + (h - a.heads)) * D + d0) =
-                        make_uint4(narrow(tag, y[0], y[1]), narrow(tag, y[2], y[3]), narrow(tag, y[4], y[5]), narrow(tag, y[6], y[7]));
+            for (int k = 0; k < 4; ++k) q[k] = fma2(u[k], inv2, magic);
+            if (kind == 2 || (a.q_weight == nullptr && a.positions == nullptr)) {
+                // rows that are only quantised get exactly the per-token quantiser: a quotient next to a tie is divided
+                const f32x2 nm = pack2(-12582912.f, -12582912.f);
+                float off = 0.f;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const f32x2 n = add2(q[k], nm), d = fma2(u[k], inv2, pack2(-n.x, -n.y));
+                    off = max3(off, fabsf(d.x), fabsf(d.y));
+                }
+                if (off > 0.4999f) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        q[k] = pack2(rintf(__fdiv_rn(u[k].x, scale)) + 12582912.f, rintf(__fdiv_rn(u[k].y, scale)) + 12582912.f);
+                }
+            }
+            if (h < count) {
+                const long long at = t * total + head0 + h;
+                const uint32_t b0 = prmt(__float_as_uint(q[0].x), __float_as_uint(q[0].y), 0x0040), b1 = prmt(__float_as_uint(q[1].x), __float_as_uint(q[1].y), 0x0040);
+                const uint32_t b2 = prmt(__float_as_uint(q[2].x), __float_as_uint(q[2].y), 0x0040), b3 = prmt(__float_as_uint(q[3].x), __float_as_uint(q[3].y), 0x0040);
+                *reinterpret_cast<uint2*>(a.codes + at * D + d0) = make_uint2(prmt(b0, b1, 0x5410), prmt(b2, b3, 0x5410));
+                if (sub == 0) a.scales[at] = scale;
+                if (kind == 1 && a.k_out != nullptr) {
+                    const f32x2 r2 = pack2(r, r);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], r2);
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (t * a.kv_heads + h) * D + d0) =
+                        make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
                 }
             }
         }
@@ -204,10 +243,10 @@ qk_norm_rope_kernel(const QkArgs a) {
 template <typename T, bool QUANT>
 int launch_qk(QkArgs a, int D, cudaStream_t st) {
     const int per_warp = kRows * (256 / D);          // rows of one token a warp takes
-    const int total = a.heads + a.kv_heads * (QUANT ? 2 : 1);
-    a.units = (total + per_warp - 1) / per_warp;
-    const long long warps = a.tokens * a.units;
-    const long long blocks = (warps + kThreads / 32 - 1) / (kThreads / 32);
+    a.q_units = (a.heads + per_warp - 1) / per_warp;
+    a.k_units = (a.kv_heads + per_warp - 1) / per_warp;
+    a.units = a.q_units + a.k_units * (QUANT ? 2 : 1);
+    const long long blocks = (a.tokens + kThreads / 32 - 1) / (kThreads / 32) * a.units;
     I8TK_REQUIRE(blocks < (1ll << 31), I8TK_ERR_UNSUPPORTED, "too many tokens");
     const dim3 grid((unsigned)blocks), block(kThreads);
     if (D == 64) I8TK_CUDA(launch_after(qk_norm_rope_kernel<T, 64, QUANT>, grid, block, 0, st, a));
@@ -246,7 +285,7 @@ extern "C" int i8tk_qk_norm_rope(const void* qkv, int dtype, int64_t row_stride,
                                  int interleaved, float eps, void* out, int64_t tokens, int heads, int kv_heads,
                                  int head_dim, i8tk_stream_t stream) {
     QkArgs a{qkv, row_stride, q_weight, k_weight, positions, rope_table, rope_rows, rotary_dim, interleaved, eps, tokens,
-             heads, kv_heads, 0, out, nullptr, nullptr, nullptr};
+             heads, kv_heads, 0, 0, 0, out, nullptr, nullptr, nullptr};
     const int rc = check_qk(a, dtype, head_dim);
     if (rc != I8TK_OK) return rc;
     I8TK_REQUIRE(out != nullptr, I8TK_ERR_INVALID_ARGUMENT, "null pointer argument");
@@ -260,7 +299,7 @@ extern "C" int i8tk_qk_norm_rope_quantize(const void* qkv, int dtype, int64_t ro
                                           float* scales, void* k_out, int64_t tokens, int heads, int kv_heads,
                                           int head_dim, i8tk_stream_t stream) {
     QkArgs a{qkv, row_stride, q_weight, k_weight, positions, rope_table, rope_rows, rotary_dim, interleaved, eps, tokens,
-             heads, kv_heads, 0, nullptr, codes, scales, k_out};
+             heads, kv_heads, 0, 0, 0, nullptr, codes, scales, k_out};
     const int rc = check_qk(a, dtype, head_dim);
     if (rc != I8TK_OK) return rc;
     I8TK_REQUIRE(codes && scales, I8TK_ERR_INVALID_ARGUMENT, "null pointer argument");
