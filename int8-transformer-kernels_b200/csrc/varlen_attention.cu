@@ -24,6 +24,7 @@
 #include "tcgen05.cuh"
 
 #include <cmath>
+#include <type_traits>
 
 namespace i8tk {
 namespace {
@@ -80,7 +81,7 @@ struct Packed {
     int B, T, max_len, causal;
     int heads, kv_heads, group;
     int tokens;                  // query tokens per CTA: floor(128 / group)
-    int slots;                   // of 64 positions in the pre-pass's arrays: T / 64 + B + 1
+    int slots;                   // of 64 positions in the pre-pass's arrays: T / 64 + B, and two behind the last
     const float* sQ;
     long long sq_stride;
     const float* sK;             // pre-pass: [kv_heads][slots * 64]
@@ -89,6 +90,7 @@ struct Packed {
     __half* out;                 // [T][heads][D]
     float score_scale_log2;
     uint32_t* status;
+    uint32_t* counter;           // work taken so far (head_dim 64 and 128); the pre-pass sets it to zero
 };
 
 // The sequence that owns slot `slot` of n-token slots, its first row and length, and the slot's place in it.  Values of
@@ -129,7 +131,10 @@ varlen_prepare_kernel(const int8_t* __restrict__ V, long long v_stride, const fl
     pdl_wait();
     pdl_launch_dependents();
     const int slot = blockIdx.x, h = blockIdx.y;
-    if (slot == 0 && h == 0 && threadIdx.x == 0) clear_call_status(a.status);
+    if (slot == 0 && h == 0 && threadIdx.x == 0) {
+        clear_call_status(a.status);
+        *a.counter = 0u;
+    }
     const Seq s = find_sequence(a.cu, a.B, a.T, a.max_len, slot, KT);
     const int valid = s.local < 0 ? 0 : min(KT, s.len - s.local * KT);      // positions of the slot that exist
     const long long row0 = (long long)s.start + (long long)s.local * KT;
@@ -557,6 +562,445 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
     }
 }
 
+// ---- head_dim 64 and 128: two query tiles per CTA, a thread per row -------------------------------------------
+// One persistent CTA per SM holds two query tiles (A and B, 128 rows each) against the same key tiles of 128
+// positions.  Each tile has its own score block and accumulator in tensor memory and its own four softmax warps, a
+// thread per row: no row is shared between threads, so nothing is exchanged, and what a tile costs besides its scores
+// (barriers, waits, the check of the maximum) is paid once per 128 scores of a thread.  While the softmax of one tile
+// runs, the tensor core works for the other.  P overwrites the scores it came from: Q.K^T of the next key tile follows
+// P.V in the order of the one thread that issues both.
+// The exponentials are taken against the reference of the tiles before, without looking for the maximum first; the
+// maximum is found on the way, and only where it runs more than kLazyStep ahead (the scores are still there) is the
+// reference moved, the accumulator rescaled and the tile done again.  The first reference of a row comes from its first
+// 32 scores.
+// The pairs of tiles are taken from a counter, long rows first, by the thread that starts the loads, which runs ahead
+// into the next pair while the last one is finished.
+constexpr int kWideThreads = 12 * 32;    // 2 x 4 softmax warps, loads, MMA, and two that fill their warpgroup
+// Registers per thread: 168 at launch; the warpgroup of loads and MMA hands most of its own to the softmax warpgroups
+// (2 * 128 * 224 + 128 * 56 = 384 * 168).
+constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
+static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kWideThreads * 168, "more registers than the block was launched with");
+constexpr int kWideKT = 128;
+constexpr int kScaleRing = 4;
+#ifndef CW
+#define CW 16
+#endif
+__device__ __forceinline__ void tmem_ldw(uint32_t a, uint32_t (&r)[16]) { tmem_ld16(a, r); }
+__device__ __forceinline__ void tmem_ldw(uint32_t a, uint32_t (&r)[32]) { tmem_ld32(a, r); }
+
+template <int D>
+struct WideCfg {
+    static constexpr int Q_BYTES = kQT * D;                                     // one query tile, one swizzled slab
+    static constexpr int K_BYTES = kWideKT * D;
+    static constexpr int V_BYTES = kWideKT * D * 2;
+    static constexpr int V_SLAB = kWideKT * 128;
+    static constexpr int OFF_Q = 0;                                             // [2 pairs][A, B]
+    static constexpr int OFF_K = OFF_Q + 4 * Q_BYTES;
+    static constexpr int OFF_V = OFF_K + kRing * K_BYTES;
+    static constexpr int OFF_SCALES = OFF_V + kRing * V_BYTES;                  // [kScaleRing]{sK[128], sV[128]}
+    static constexpr int OFF_BARS = OFF_SCALES + kScaleRing * 2 * kWideKT * 4;
+    static constexpr int NUM_BARS = 40;
+    static constexpr int SMEM_BYTES = 1024 + OFF_BARS + NUM_BARS * 8 + 16;
+    static constexpr int TM_S = 0;                                              // A, B: 128 columns each; P in the first 64
+    static constexpr int TM_O = 256;                                            // A, B: D columns each
+    static_assert(SMEM_BYTES + 1024 <= 227 * 1024, "shared memory of an SM");
+};
+enum WideBar : int {
+    W_WFULL = 0,      // [2]
+    W_WEMPTY = 2,     // [2]
+    W_QFULL = 4,      // [2]
+    W_QEMPTY = 6,     // [2]
+    W_KFULL = 8,      // [kRing]
+    W_KEMPTY = 11,    // [kRing]
+    W_VFULL = 14,     // [kRing]
+    W_VEMPTY = 17,    // [kRing]
+    W_CFULL = 20,     // [kScaleRing]
+    W_CEMPTY = 24,    // [kScaleRing]
+    W_SFULL = 28,     // [A, B]
+    W_PFULL = 30,     // [A, B]
+    W_ODONE = 32,     // [A, B]
+    W_OEMPTY = 34,    // [A, B]
+};
+struct WideWork {
+    int start, len, tok0, hk, kv_slot, nt_a, nt_b, pad;      // nt_a < 0: no more work
+};
+
+template <int D>
+__global__ void __launch_bounds__(kWideThreads, 1)
+varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Packed a) {
+    using Cfg = WideCfg<D>;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ WideWork work[2];
+    const uint32_t raw_s = smem_u32(smem_raw);
+    const uint32_t base_s = (raw_s + 1023u) & ~1023u;       // swizzle patterns are functions of address bits
+    unsigned char* base = smem_raw + (base_s - raw_s);
+    const uint32_t bars = base_s + Cfg::OFF_BARS;
+    auto bar = [&](int i) -> uint32_t { return bars + 8u * i; };
+    const uint32_t tmem_slot = bars + Cfg::NUM_BARS * 8;
+    volatile uint32_t* tmem_slot_p = reinterpret_cast<volatile uint32_t*>(base + Cfg::OFF_BARS + Cfg::NUM_BARS * 8);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(bar(W_WFULL + i), 1);
+            mbar_init(bar(W_WEMPTY + i), 9);
+            mbar_init(bar(W_QFULL + i), 1);
+            mbar_init(bar(W_QEMPTY + i), 1);
+            mbar_init(bar(W_SFULL + i), 1);
+            mbar_init(bar(W_PFULL + i), 4);
+            mbar_init(bar(W_ODONE + i), 1);
+            mbar_init(bar(W_OEMPTY + i), 4);
+        }
+        for (int i = 0; i < kRing; ++i) {
+            mbar_init(bar(W_KFULL + i), 1);
+            mbar_init(bar(W_KEMPTY + i), 1);
+            mbar_init(bar(W_VFULL + i), 1);
+            mbar_init(bar(W_VEMPTY + i), 1);
+        }
+        for (int i = 0; i < kScaleRing; ++i) {
+            mbar_init(bar(W_CFULL + i), 1);
+            mbar_init(bar(W_CEMPTY + i), 8);
+        }
+        fence_mbar_init();
+    }
+    if (warp == 9) tmem_alloc(tmem_slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot_p;
+    pdl_wait();
+    pdl_launch_dependents();
+    const int two = 2 * a.tokens;                            // query tokens of a pair of tiles
+
+    // (each split in its own branch: where the two meet, the compiler has the smaller one)
+    if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == 8) {
+        // ================= work and loads =================
+        if (lane == 0) {
+            const int slots = a.T / two + a.B, items = slots * a.kv_heads;
+            bool ok = true;
+            int t = 0;                                       // key tiles loaded so far
+            int next = (int)atomicAdd(a.counter, 1u);
+            for (int w = 0; ok; ++w) {
+                WideWork x;
+                x.nt_a = -1;
+                for (;;) {                                   // to a slot that has rows
+                    const int item = next;
+                    if (item >= items) break;
+                    next = (int)atomicAdd(a.counter, 1u);
+                    x.hk = item % a.kv_heads;
+                    const Seq s = find_sequence(a.cu, a.B, a.T, a.max_len, slots - 1 - item / a.kv_heads, two);
+                    x.start = s.start, x.len = s.len, x.tok0 = s.local * two;
+                    if (s.local < 0 || x.tok0 >= s.len) continue;
+                    x.kv_slot = s.start / KT + (s.first_slot - s.start / two);
+                    auto tiles = [&](int tok) {              // key tiles of the query tile that begins at this token
+                        return tok >= s.len ? 0 : ((a.causal ? min(s.len, tok + a.tokens) : s.len) + kWideKT - 1) / kWideKT;
+                    };
+                    x.nt_a = tiles(x.tok0), x.nt_b = tiles(x.tok0 + a.tokens);
+                    break;
+                }
+                const int ws = w & 1;
+                const uint32_t round = (uint32_t)(w >> 1) & 1u;
+                if (!mbar_wait_bounded(bar(W_WEMPTY + ws), round ^ 1u)) { ok = false; break; }
+                work[ws] = x;
+                mbar_arrive(bar(W_WFULL + ws));
+                if (x.nt_a < 0) break;
+                if (!mbar_wait_bounded(bar(W_QEMPTY + ws), round ^ 1u)) { ok = false; break; }
+                const int q_rows = a.tokens * a.group * D, q_at = base_s + Cfg::OFF_Q + ws * 2 * Cfg::Q_BYTES;
+                mbar_expect_tx(bar(W_QFULL + ws), x.nt_b > 0 ? 2 * q_rows : q_rows);
+                tma_load_3d(q_at, &tmQ, 0, x.hk * a.group, x.start + x.tok0, bar(W_QFULL + ws));
+                if (x.nt_b > 0) tma_load_3d(q_at + Cfg::Q_BYTES, &tmQ, 0, x.hk * a.group, x.start + x.tok0 + a.tokens, bar(W_QFULL + ws));
+                const int nt = max(x.nt_a, x.nt_b);
+                const long long sc0 = ((long long)x.hk * a.slots + x.kv_slot) * KT;
+                for (int j = 0; j < nt; ++j, ++t) {
+                    const int st = t % kRing, cs = t % kScaleRing;
+                    const uint32_t r = ((uint32_t)(t / kRing) & 1u) ^ 1u, cr = ((uint32_t)(t / kScaleRing) & 1u) ^ 1u;
+                    if (!mbar_wait_bounded(bar(W_KEMPTY + st), r) || !mbar_wait_bounded(bar(W_CEMPTY + cs), cr)) { ok = false; break; }
+                    mbar_expect_tx(bar(W_KFULL + st), Cfg::K_BYTES);
+                    tma_load_3d(base_s + Cfg::OFF_K + st * Cfg::K_BYTES, &tmK, 0, x.hk, x.start + j * kWideKT, bar(W_KFULL + st));
+                    mbar_expect_tx(bar(W_CFULL + cs), 2 * kWideKT * 4);
+                    const uint32_t c_at = base_s + Cfg::OFF_SCALES + cs * (2 * kWideKT * 4);
+                    bulk_g2s(c_at, a.sK + sc0 + j * kWideKT, kWideKT * 4, bar(W_CFULL + cs));
+                    bulk_g2s(c_at + kWideKT * 4, a.sV + sc0 + j * kWideKT, kWideKT * 4, bar(W_CFULL + cs));
+                    if (!mbar_wait_bounded(bar(W_VEMPTY + st), r)) { ok = false; break; }
+                    mbar_expect_tx(bar(W_VFULL + st), Cfg::V_BYTES);
+#pragma unroll
+                    for (int sl = 0; sl < D / 64; ++sl)
+                        tma_load_2d(base_s + Cfg::OFF_V + st * Cfg::V_BYTES + sl * Cfg::V_SLAB, &tmV, sl * 128,
+                                    (int)(sc0 + j * kWideKT), bar(W_VFULL + st));
+                }
+            }
+            if (!ok) {                                       // copies in flight land before the block lets go of its memory
+                note_timeout(a.status);
+                for (int i = 0; i < kRing; ++i)
+                    for (uint32_t ph = 0; ph < 2; ++ph)
+                        mbar_wait_bounded(bar(W_KFULL + i), ph, 64u), mbar_wait_bounded(bar(W_VFULL + i), ph, 64u);
+            }
+        }
+    } else if (warp == 9) {
+        // ================= MMA issuer =================
+        if (elect_one()) {
+            constexpr uint32_t idesc_qk = idesc_i8(kQT, kWideKT);
+            constexpr uint32_t idesc_pv = idesc_f16(kQT, D, true);
+            bool ok = true;
+            int t0 = 0;                                      // key tiles of the pairs before
+            uint32_t n_p[2] = {0u, 0u}, n_o[2] = {0u, 0u};   // softmax tiles and accumulators waited for
+            for (int w = 0; ok; ++w) {
+                const int ws = w & 1;
+                const uint32_t round = (uint32_t)(w >> 1) & 1u;
+                if (!mbar_wait_spin_bounded(bar(W_WFULL + ws), round)) { ok = false; break; }
+                const int nt_a = work[ws].nt_a, nt_b = work[ws].nt_b;
+                mbar_arrive(bar(W_WEMPTY + ws));
+                if (nt_a < 0) break;
+                const int nt = max(nt_a, nt_b);
+                if (!mbar_wait_spin_bounded(bar(W_QFULL + ws), round)) { ok = false; break; }
+                auto qk = [&](int x, int j) {                // scores of tile x against key tile j
+                    const uint32_t qa = base_s + Cfg::OFF_Q + (ws * 2 + x) * Cfg::Q_BYTES;
+                    const uint32_t ka = base_s + Cfg::OFF_K + ((t0 + j) % kRing) * Cfg::K_BYTES;
+                    const uint64_t da = D == 128 ? smem_desc_sw128(qa) : smem_desc_sw64(qa);
+                    const uint64_t db = D == 128 ? smem_desc_sw128(ka) : smem_desc_sw64(ka);
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) mma_i8(tmem_base + Cfg::TM_S + x * 128, da + 2 * k, db + 2 * k, idesc_qk, k != 0);
+                    tc_commit(bar(W_SFULL + x));
+                };
+                // A's and B's turn at key tile j: P.V of j, then Q.K^T of j + 1 into the scores' place
+                for (int j = -1; j < nt && ok; ++j) {
+                    if (j + 1 < nt && !mbar_wait_spin_bounded(bar(W_KFULL + (t0 + j + 1) % kRing), (uint32_t)((t0 + j + 1) / kRing) & 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    if (j >= 0 && !mbar_wait_spin_bounded(bar(W_VFULL + (t0 + j) % kRing), (uint32_t)((t0 + j) / kRing) & 1u)) {
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const int mine = x == 0 ? nt_a : nt_b;
+                        if (j >= 0 && j < mine) {
+                            if (!mbar_wait_spin_bounded(bar(W_PFULL + x), n_p[x] & 1u)) { ok = false; break; }
+                            ++n_p[x];
+                            if (j == 0) {                    // the accumulator of the pair before has been read
+                                if (!mbar_wait_spin_bounded(bar(W_OEMPTY + x), (n_o[x] & 1u) ^ 1u)) { ok = false; break; }
+                                ++n_o[x];
+                            }
+                            tc_fence_after();
+                            const uint64_t db0 = smem_desc_sw128_mn(base_s + Cfg::OFF_V + ((t0 + j) % kRing) * Cfg::V_BYTES, Cfg::V_SLAB);
+#pragma unroll
+                            for (int i = 0; i < kWideKT / 16; ++i)
+                                mma_f16_ta(tmem_base + Cfg::TM_O + x * D, tmem_base + Cfg::TM_S + x * 128 + i * 8, db0 + (uint64_t)(128 * i),
+                                           idesc_pv, (j | i) != 0);
+                            if (j + 1 == mine) tc_commit(bar(W_ODONE + x));
+                        }
+                        if (j + 1 < mine) qk(x, j + 1);
+                    }
+                    if (!ok) break;
+                    if (j + 1 < nt) tc_commit(bar(W_KEMPTY + (t0 + j + 1) % kRing));
+                    if (j >= 0) tc_commit(bar(W_VEMPTY + (t0 + j) % kRing));
+                }
+                tc_commit(bar(W_QEMPTY + ws));
+                t0 += nt;
+            }
+            if (!ok) note_timeout(a.status);
+        }
+    }
+    } else {
+        // ================= softmax: a query row per thread =================
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+        const int x = warp >> 2;                             // tile A or B
+        const int r = (warp & 3) * 32 + lane;                // row of the tile; the warp's quarter of the lanes of tensor memory
+        const uint32_t lane_addr = tmem_base + ((uint32_t)((warp & 3) * 32) << 16);
+        const uint32_t s_addr = lane_addr + Cfg::TM_S + x * 128, o_addr = lane_addr + Cfg::TM_O + x * D;
+        constexpr uint32_t kMagicI = 0x4B400000u;            // 1.5 * 2^23: |q.k| < 2^22 converts by an add and a subtract
+        const f32x2 nmagic2 = pack2(-12582912.f, -12582912.f);
+        bool ok = true;
+        int t0 = 0;
+        uint32_t n_s = 0u, n_o = 0u;                         // score blocks and accumulators waited for
+        for (int w = 0; ok; ++w) {
+            const int ws = w & 1;
+            const uint32_t round = (uint32_t)(w >> 1) & 1u;
+            ok = __all_sync(0xffffffffu, mbar_wait_spin_bounded(bar(W_WFULL + ws), round));
+            if (!ok) break;
+            const WideWork job = work[ws];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(W_WEMPTY + ws));
+            if (job.nt_a < 0) break;
+            const int nt = max(job.nt_a, job.nt_b), mine = x == 0 ? job.nt_a : job.nt_b;
+            const int first_tok = job.tok0 + x * a.tokens;
+            const int tok = first_tok + r / a.group, head = job.hk * a.group + r % a.group;
+            const bool stored = r < a.tokens * a.group && tok < job.len;
+            float qscale = stored ? a.sQ[(long long)(job.start + tok) * a.sq_stride + head] * a.score_scale_log2 : 0.f;
+            if (qscale == 0.f) qscale = 1e-30f;              // a removed position (-inf) stays removed under a scale of zero
+            const f32x2 qs2 = pack2(qscale, qscale);
+            const int visible = a.causal ? min(job.len, tok + 1) : job.len;             // positions that this row sees
+            const int all_visible = a.causal ? first_tok + 1 : job.len;                 // that every row of the tile sees
+            // the power of two that brings the largest value scale of the sequence to [2^6, 2^7), as an addend of the
+            // exponent: it cancels against the sum of the probabilities
+            float most = 0.f;
+            const int top_slots = ((a.causal ? min(job.len, first_tok + a.tokens) : job.len) + KT - 1) / KT;
+            for (int j = lane; j < top_slots && mine > 0; j += 32) most = fmaxf(most, a.top[(long long)job.hk * a.slots + job.kv_slot + j]);
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+            const float lift = (float)min(100, max(-100, 6 - ((int)(__float_as_uint(most) >> 23) - 127)));
+
+            float nm = 0.f;                                  // lift less the reference (log2 units)
+            float l = 0.f;
+            for (int j = 0; j < nt; ++j) {
+                const int cs = (t0 + j) % kScaleRing;
+                ok = __all_sync(0xffffffffu, mbar_wait_spin_bounded(bar(W_CFULL + cs), (uint32_t)((t0 + j) / kScaleRing) & 1u));
+                if (!ok) break;
+                if (j < mine) {
+                    ok = __all_sync(0xffffffffu, mbar_wait_spin_bounded(bar(W_SFULL + x), n_s & 1u));
+                    if (!ok) break;
+                    ++n_s;
+                    tc_fence_after();
+                    const float* sk = reinterpret_cast<const float*>(base + Cfg::OFF_SCALES) + cs * (2 * kWideKT);
+                    const float* sv = sk + kWideKT;
+                    const int lim = visible - j * kWideKT;               // columns of this tile that the row sees
+                    const bool edge = (j + 1) * kWideKT > all_visible;   // (the same for the whole tile)
+                    // y = (q.k) * sK for 8 columns; columns the row does not see are removed, whatever was there
+                    auto scores8 = [&](auto at_edge, const uint32_t* sr8, int c, f32x2* y4) {
+                        const float4 ka = *reinterpret_cast<const float4*>(sk + c), kb = *reinterpret_cast<const float4*>(sk + c + 4);
+                        const f32x2 t01 = add2(pack2(__uint_as_float(sr8[0] + kMagicI), __uint_as_float(sr8[1] + kMagicI)), nmagic2);
+                        const f32x2 t23 = add2(pack2(__uint_as_float(sr8[2] + kMagicI), __uint_as_float(sr8[3] + kMagicI)), nmagic2);
+                        const f32x2 t45 = add2(pack2(__uint_as_float(sr8[4] + kMagicI), __uint_as_float(sr8[5] + kMagicI)), nmagic2);
+                        const f32x2 t67 = add2(pack2(__uint_as_float(sr8[6] + kMagicI), __uint_as_float(sr8[7] + kMagicI)), nmagic2);
+                        y4[0] = mul2(t01, pack2(ka.x, ka.y));
+                        y4[1] = mul2(t23, pack2(ka.z, ka.w));
+                        y4[2] = mul2(t45, pack2(kb.x, kb.y));
+                        y4[3] = mul2(t67, pack2(kb.z, kb.w));
+                        if constexpr (decltype(at_edge)::value) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if (c + 2 * e >= lim) y4[e].x = -INFINITY;
+                                if (c + 2 * e + 1 >= lim) y4[e].y = -INFINITY;
+                            }
+                        }
+                    };
+                    if (j == 0) {                            // the first reference: largest of the first 32 scores
+                        uint32_t sr[32];
+                        float m0 = -INFINITY;
+                        tmem_ld32(s_addr, sr);
+                        tmem_ld_wait(sr);
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            f32x2 y4[4];
+                            scores8(std::true_type{}, &sr[8 * g], 8 * g, y4);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) m0 = max3(m0, y4[e].x, y4[e].y);
+                        }
+                        nm = lift - m0 * qscale;
+                        if (!(fabsf(nm) < 1e30f)) nm = lift; // (scores that are not finite: the row becomes NaN by itself)
+                    }
+                    uint32_t P[64];
+                    f32x2 sum2;
+                    float mx;
+                    auto pass = [&](auto at_edge) {
+                        const f32x2 nm2 = pack2(nm, nm);
+                        sum2 = pack2(0.f, 0.f);
+                        mx = -INFINITY;
+                        uint32_t sr[2][CW];
+                        tmem_ldw(s_addr, sr[0]);
+#pragma unroll
+                        for (int c = 0; c < 128 / CW; ++c) {
+                            tmem_ld_wait(sr[c & 1]);
+                            if (c < 128 / CW - 1) tmem_ldw(s_addr + (c + 1) * CW, sr[(c + 1) & 1]);
+#pragma unroll
+                            for (int g = 0; g < CW / 8; ++g) {
+                                const int col = c * CW + g * 8;
+                                f32x2 y4[4];
+                                scores8(at_edge, &sr[c & 1][8 * g], col, y4);
+                                const float4 va = *reinterpret_cast<const float4*>(sv + col), vb = *reinterpret_cast<const float4*>(sv + col + 4);
+                                const f32x2 x0 = fma2(y4[0], qs2, nm2), x1 = fma2(y4[1], qs2, nm2);
+                                const f32x2 x2 = fma2(y4[2], qs2, nm2), x3 = fma2(y4[3], qs2, nm2);
+                                mx = max3(max3(mx, x0.x, x0.y), max3(x1.x, x1.y, x2.x), fmaxf(x2.y, fmaxf(x3.x, x3.y)));
+                                const f32x2 p0 = pack2(ex2_approx(x0.x), ex2_approx(x0.y)), p1 = pack2(ex2_approx(x1.x), ex2_approx(x1.y));
+                                const f32x2 p2 = pack2(ex2_approx(x2.x), ex2_approx(x2.y)), p3 = pack2(ex2_approx(x3.x), ex2_approx(x3.y));
+                                sum2 = add2(sum2, add2(add2(p0, p1), add2(p2, p3)));
+                                const f32x2 s0 = mul2(p0, pack2(va.x, va.y)), s1 = mul2(p1, pack2(va.z, va.w));
+                                const f32x2 s2 = mul2(p2, pack2(vb.x, vb.y)), s3 = mul2(p3, pack2(vb.z, vb.w));
+                                P[col / 2] = pack_h2(s0.x, s0.y), P[col / 2 + 1] = pack_h2(s1.x, s1.y);
+                                P[col / 2 + 2] = pack_h2(s2.x, s2.y), P[col / 2 + 3] = pack_h2(s3.x, s3.y);
+                            }
+                        }
+                    };
+                    for (;;) {
+                        if (edge) pass(std::true_type{});
+                        else pass(std::false_type{});
+                        const bool ahead = mx > lift + kLazyStep;
+                        if (!__any_sync(0xffffffffu, ahead)) break;
+                        // the reference moves to this tile's maximum, and the tile is done again; P.V of the tile before
+                        // has retired (its commit came before that of these scores)
+                        const float up = ahead ? mx - lift : 0.f, corr = ex2_approx(-up);
+                        nm -= up;
+                        l *= corr;
+                        if (j > 0) {
+                            uint32_t o[32];
+#pragma unroll 1
+                            for (int cc = 0; cc < D / 32; ++cc) {
+                                tmem_ld32(o_addr + cc * 32, o);
+                                tmem_ld_wait(o);
+#pragma unroll
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+                                tmem_st32(o_addr + cc * 32, o);
+                            }
+                        }
+                    }
+                    l += sum2.x + sum2.y;
+                    tmem_st32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&P[0]));
+                    tmem_st32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&P[32]));
+                    tmem_st_wait();
+                    tc_fence_before();
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bar(W_CEMPTY + cs));
+                    if (j < mine) mbar_arrive(bar(W_PFULL + x));
+                }
+            }
+            t0 += nt;
+            // ---- epilogue: O / l -> fp16 ----
+            if (ok && mine > 0) {
+                ok = __all_sync(0xffffffffu, mbar_wait_spin_bounded(bar(W_ODONE + x), n_o & 1u));
+                if (!ok) break;
+                ++n_o;
+                tc_fence_after();
+                const float inv = 1.0f / l;
+                __half* orow = a.out + ((long long)(job.start + tok) * a.heads + head) * D;
+#pragma unroll 1
+                for (int cc = 0; cc < D / 32; ++cc) {
+                    uint32_t o[32];
+                    tmem_ld32(o_addr + cc * 32, o);
+                    tmem_ld_wait(o);
+                    if (stored) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            *reinterpret_cast<uint4*>(orow + cc * 32 + k * 8) =
+                                make_uint4(pack_h2(__uint_as_float(o[8 * k]) * inv, __uint_as_float(o[8 * k + 1]) * inv),
+                                           pack_h2(__uint_as_float(o[8 * k + 2]) * inv, __uint_as_float(o[8 * k + 3]) * inv),
+                                           pack_h2(__uint_as_float(o[8 * k + 4]) * inv, __uint_as_float(o[8 * k + 5]) * inv),
+                                           pack_h2(__uint_as_float(o[8 * k + 6]) * inv, __uint_as_float(o[8 * k + 7]) * inv));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar(W_OEMPTY + x));
+            }
+        }
+        if (!ok && lane == 0) note_timeout(a.status);
+    }
+
+    // common exit: every role ends here, then the allocating warp frees tensor memory
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_dealloc(tmem_base, 512);
+    }
+}
+
 // ---- host ----------------------------------------------------------------------------------------------
 // [rows][heads][D] bytes with `stride` bytes between rows: boxes of box_rows x box_heads x box_bytes
 int encode_heads(CUtensorMap* map, const void* ptr, unsigned long long rows, unsigned heads, unsigned D, unsigned long long stride,
@@ -577,7 +1021,7 @@ struct VarLayout {
 };
 VarLayout var_layout(long long T, long long B, int kv_heads, int D) {
     VarLayout y;
-    y.slots = (int)(T / KT + B + 1);
+    y.slots = (int)(T / KT + B + 2);
     const size_t rows = (size_t)kv_heads * y.slots * KT;
     y.sk_off = 256;
     y.sv_off = y.sk_off + round_up(rows * 4, 256);
@@ -590,7 +1034,7 @@ bool var_shape_ok(long long T, long long B, int heads, int kv_heads, int D) {
     if (T <= 0 || B <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads != 0 || heads / kv_heads > 64 || (D != 64 && D != 128 && D != 256))
         return false;
     const int tokens = kQT / (heads / kv_heads);
-    return T < (1ll << 30) && B < (1ll << 28) && kv_heads <= 65535 && (T / KT + B + 1) * kv_heads * KT < (1ll << 31) &&
+    return T < (1ll << 30) && B < (1ll << 28) && kv_heads <= 65535 && (T / KT + B + 2) * kv_heads * KT < (1ll << 31) &&
            (T / tokens + B + 1) * kv_heads < (1ll << 31);
 }
 
@@ -598,13 +1042,21 @@ template <int D>
 int launch_varlen(const int8_t* Q, long long q_stride, const int8_t* K, long long k_stride, const int8_t* V, long long v_stride,
                   const float* sK, long long sk_stride, const float* sV, long long sv_stride, Packed a, unsigned char* ws,
                   cudaStream_t st) {
-    using Cfg = VarCfg<D>;
-    static bool attr_done[64] = {false};
+    constexpr bool kWide = D <= 128;
+    constexpr int KEYS = kWide ? kWideKT : KT;               // positions of a key tile
+    constexpr int ROW = D < 128 ? D : 128;
+    static int sms[64] = {0};
     int dev = 0;
     I8TK_CUDA(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-        I8TK_CUDA(cudaFuncSetAttribute(varlen_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg::SMEM_BYTES));
-        if (dev >= 0 && dev < 64) attr_done[dev] = true;
+    I8TK_REQUIRE(dev >= 0 && dev < 64, I8TK_ERR_UNSUPPORTED, "device %d", dev);
+    if (sms[dev] == 0) {
+        int n = 0;
+        I8TK_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+        if constexpr (kWide)
+            I8TK_CUDA(cudaFuncSetAttribute(varlen_wide_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideCfg<D>::SMEM_BYTES));
+        else
+            I8TK_CUDA(cudaFuncSetAttribute(varlen_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, VarCfg<D>::SMEM_BYTES));
+        sms[dev] = n;
     }
     const VarLayout y = var_layout(a.T, a.B, a.kv_heads, D);
     float* sKp = reinterpret_cast<float*>(ws + y.sk_off);
@@ -616,17 +1068,23 @@ int launch_varlen(const int8_t* Q, long long q_stride, const int8_t* K, long lon
 
     const CUtensorMapSwizzle sw = (D >= 128) ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     CUtensorMap tmQ, tmK, tmV;
-    int rc = encode_heads(&tmQ, Q, a.T, a.heads, D, q_stride, a.tokens, a.group, Cfg::ROW_BYTES, sw);
+    int rc = encode_heads(&tmQ, Q, a.T, a.heads, D, q_stride, a.tokens, a.group, ROW, sw);
     I8TK_REQUIRE(rc == 0, I8TK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", rc);
-    rc = encode_heads(&tmK, K, a.T, a.kv_heads, D, k_stride, KT, 1, Cfg::ROW_BYTES, sw);
+    rc = encode_heads(&tmK, K, a.T, a.kv_heads, D, k_stride, KEYS, 1, ROW, sw);
     I8TK_REQUIRE(rc == 0, I8TK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", rc);
-    rc = encode_map_2d_u8(&tmV, V16, (unsigned long long)a.kv_heads * a.slots * KT, 2ull * D, KT, 128, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = encode_map_2d_u8(&tmV, V16, (unsigned long long)a.kv_heads * a.slots * KT, 2ull * D, KEYS, 128, CU_TENSOR_MAP_SWIZZLE_128B);
     I8TK_REQUIRE(rc == 0, I8TK_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", rc);
 
     I8TK_CUDA(launch_after(varlen_prepare_kernel<D>, dim3((unsigned)a.slots, (unsigned)a.kv_heads), dim3(128), 0, st, V, v_stride, sK,
                            sk_stride, sV, sv_stride, V16, sKp, sVp, top, a));
-    const unsigned ctas = (unsigned)((a.T / a.tokens + a.B) * (long long)a.kv_heads);
-    I8TK_CUDA(launch_after(varlen_attention_kernel<D>, dim3(ctas), dim3(kThreads), Cfg::SMEM_BYTES, st, tmQ, tmK, tmV, a));
+    if constexpr (kWide) {
+        const long long items = (a.T / (2 * a.tokens) + a.B) * (long long)a.kv_heads;
+        I8TK_CUDA(launch_after(varlen_wide_kernel<D>, dim3((unsigned)(items < sms[dev] ? items : sms[dev])), dim3(kWideThreads),
+                               WideCfg<D>::SMEM_BYTES, st, tmQ, tmK, tmV, a));
+    } else {
+        const unsigned ctas = (unsigned)((a.T / a.tokens + a.B) * (long long)a.kv_heads);
+        I8TK_CUDA(launch_after(varlen_attention_kernel<D>, dim3(ctas), dim3(kThreads), VarCfg<D>::SMEM_BYTES, st, tmQ, tmK, tmV, a));
+    }
     return I8TK_OK;
 }
 
@@ -667,7 +1125,7 @@ extern "C" int i8tk_attention_varlen(const int8_t* Q, int64_t q_stride, const in
     const int group = heads / kv_heads;
     Packed a{cu_seqlens, batch, (int)tokens, max_seqlen, causal ? 1 : 0, heads, kv_heads, group, kQT / group, 0, sQ, sq_stride,
              nullptr, nullptr, nullptr, static_cast<__half*>(out_f16), 1.4426950408889634f / sqrtf((float)head_dim),
-             static_cast<uint32_t*>(workspace)};
+             static_cast<uint32_t*>(workspace), static_cast<uint32_t*>(workspace) + 2};
     unsigned char* ws = static_cast<unsigned char*>(workspace);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (head_dim == 64) return launch_varlen<64>(Q, q_stride, K, k_stride, V, v_stride, sK, sk_stride, sV, sv_stride, a, ws, st);
