@@ -582,11 +582,6 @@ constexpr int kSoftmaxRegs = 224, kOtherRegs = 56;
 static_assert(256 * kSoftmaxRegs + 128 * kOtherRegs <= kWideThreads * 168, "more registers than the block was launched with");
 constexpr int kWideKT = 128;
 constexpr int kScaleRing = 4;
-#ifndef CW
-#define CW 16
-#endif
-__device__ __forceinline__ void tmem_ldw(uint32_t a, uint32_t (&r)[16]) { tmem_ld16(a, r); }
-__device__ __forceinline__ void tmem_ldw(uint32_t a, uint32_t (&r)[32]) { tmem_ld32(a, r); }
 
 template <int D>
 struct WideCfg {
@@ -744,64 +739,72 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
         if (elect_one()) {
             constexpr uint32_t idesc_qk = idesc_i8(kQT, kWideKT);
             constexpr uint32_t idesc_pv = idesc_f16(kQT, D, true);
-            bool ok = true;
             int t0 = 0;                                      // key tiles of the pairs before
             uint32_t n_p[2] = {0u, 0u}, n_o[2] = {0u, 0u};   // softmax tiles and accumulators waited for
-            for (int w = 0; ok; ++w) {
+            // the next pair's sizes, its queries and its first keys: false when a wait gave up
+            auto take = [&](int w, int first, int (&nt)[2]) -> bool {
                 const int ws = w & 1;
                 const uint32_t round = (uint32_t)(w >> 1) & 1u;
-                if (!mbar_wait_spin_bounded(bar(W_WFULL + ws), round)) { ok = false; break; }
-                const int nt_a = work[ws].nt_a, nt_b = work[ws].nt_b;
+                if (!mbar_wait_spin_bounded(bar(W_WFULL + ws), round)) return false;
+                nt[0] = work[ws].nt_a, nt[1] = work[ws].nt_b;
                 mbar_arrive(bar(W_WEMPTY + ws));
-                if (nt_a < 0) break;
-                const int nt = max(nt_a, nt_b);
-                if (!mbar_wait_spin_bounded(bar(W_QFULL + ws), round)) { ok = false; break; }
-                auto qk = [&](int x, int j) {                // scores of tile x against key tile j
-                    const uint32_t qa = base_s + Cfg::OFF_Q + (ws * 2 + x) * Cfg::Q_BYTES;
-                    const uint32_t ka = base_s + Cfg::OFF_K + ((t0 + j) % kRing) * Cfg::K_BYTES;
-                    const uint64_t da = D == 128 ? smem_desc_sw128(qa) : smem_desc_sw64(qa);
-                    const uint64_t db = D == 128 ? smem_desc_sw128(ka) : smem_desc_sw64(ka);
+                return nt[0] < 0 || (mbar_wait_spin_bounded(bar(W_QFULL + ws), round) &&
+                                     mbar_wait_spin_bounded(bar(W_KFULL + first % kRing), (uint32_t)(first / kRing) & 1u));
+            };
+            auto qk = [&](int ws, int x, int t) {            // scores of tile x of pair slot ws against key tile t
+                tc_fence_after();
+                const uint32_t qa = base_s + Cfg::OFF_Q + (ws * 2 + x) * Cfg::Q_BYTES;
+                const uint32_t ka = base_s + Cfg::OFF_K + (t % kRing) * Cfg::K_BYTES;
+                const uint64_t da = D == 128 ? smem_desc_sw128(qa) : smem_desc_sw64(qa);
+                const uint64_t db = D == 128 ? smem_desc_sw128(ka) : smem_desc_sw64(ka);
 #pragma unroll
-                    for (int k = 0; k < D / 32; ++k) mma_i8(tmem_base + Cfg::TM_S + x * 128, da + 2 * k, db + 2 * k, idesc_qk, k != 0);
-                    tc_commit(bar(W_SFULL + x));
-                };
-                // A's and B's turn at key tile j: P.V of j, then Q.K^T of j + 1 into the scores' place
-                for (int j = -1; j < nt && ok; ++j) {
-                    if (j + 1 < nt && !mbar_wait_spin_bounded(bar(W_KFULL + (t0 + j + 1) % kRing), (uint32_t)((t0 + j + 1) / kRing) & 1u)) {
-                        ok = false;
-                        break;
-                    }
-                    if (j >= 0 && !mbar_wait_spin_bounded(bar(W_VFULL + (t0 + j) % kRing), (uint32_t)((t0 + j) / kRing) & 1u)) {
-                        ok = false;
-                        break;
-                    }
-                    tc_fence_after();
+                for (int k = 0; k < D / 32; ++k) mma_i8(tmem_base + Cfg::TM_S + x * 128, da + 2 * k, db + 2 * k, idesc_qk, k != 0);
+                tc_commit(bar(W_SFULL + x));
+            };
+            int cur[2] = {-1, -1}, then[2] = {-1, -1};       // key tiles of A and B, of this pair and of the next
+            bool ok = take(0, 0, cur);
+            if (ok && cur[0] > 0) {
+                qk(0, 0, 0);
+                if (cur[1] > 0) qk(0, 1, 0);
+                tc_commit(bar(W_KEMPTY));
+            }
+            for (int w = 0; ok && cur[0] > 0; ++w) {
+                const int ws = w & 1, nt = max(cur[0], cur[1]);
+                // A's and B's turn at key tile j: P.V of j, then Q.K^T of j + 1 -- behind the last tile, of the next pair's
+                // first -- into the scores' place
+                for (int j = 0; j < nt; ++j) {
+                    const bool last = j + 1 == nt;
+                    const int kt = t0 + j + 1, vt = t0 + j;
+                    ok = (last ? take(w + 1, kt, then) : mbar_wait_spin_bounded(bar(W_KFULL + kt % kRing), (uint32_t)(kt / kRing) & 1u)) &&
+                         mbar_wait_spin_bounded(bar(W_VFULL + vt % kRing), (uint32_t)(vt / kRing) & 1u);
 #pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const int mine = x == 0 ? nt_a : nt_b;
-                        if (j >= 0 && j < mine) {
-                            if (!mbar_wait_spin_bounded(bar(W_PFULL + x), n_p[x] & 1u)) { ok = false; break; }
+                        if (ok && j < cur[x]) {
+                            ok = mbar_wait_spin_bounded(bar(W_PFULL + x), n_p[x] & 1u);
                             ++n_p[x];
-                            if (j == 0) {                    // the accumulator of the pair before has been read
-                                if (!mbar_wait_spin_bounded(bar(W_OEMPTY + x), (n_o[x] & 1u) ^ 1u)) { ok = false; break; }
+                            if (ok && j == 0) {              // the accumulator of the pair before has been read
+                                ok = mbar_wait_spin_bounded(bar(W_OEMPTY + x), (n_o[x] & 1u) ^ 1u);
                                 ++n_o[x];
                             }
+                            if (!ok) break;
                             tc_fence_after();
-                            const uint64_t db0 = smem_desc_sw128_mn(base_s + Cfg::OFF_V + ((t0 + j) % kRing) * Cfg::V_BYTES, Cfg::V_SLAB);
+                            const uint64_t db0 = smem_desc_sw128_mn(base_s + Cfg::OFF_V + (vt % kRing) * Cfg::V_BYTES, Cfg::V_SLAB);
 #pragma unroll
                             for (int i = 0; i < kWideKT / 16; ++i)
                                 mma_f16_ta(tmem_base + Cfg::TM_O + x * D, tmem_base + Cfg::TM_S + x * 128 + i * 8, db0 + (uint64_t)(128 * i),
                                            idesc_pv, (j | i) != 0);
-                            if (j + 1 == mine) tc_commit(bar(W_ODONE + x));
+                            if (j + 1 == cur[x]) tc_commit(bar(W_ODONE + x));
                         }
-                        if (j + 1 < mine) qk(x, j + 1);
+                        if (ok && (last ? then[x] > 0 : j + 1 < cur[x])) qk(last ? ws ^ 1 : ws, x, kt);
                     }
                     if (!ok) break;
-                    if (j + 1 < nt) tc_commit(bar(W_KEMPTY + (t0 + j + 1) % kRing));
-                    if (j >= 0) tc_commit(bar(W_VEMPTY + (t0 + j) % kRing));
+                    if (!last || then[0] > 0) tc_commit(bar(W_KEMPTY + kt % kRing));
+                    tc_commit(bar(W_VEMPTY + vt % kRing));
                 }
+                if (!ok) break;
                 tc_commit(bar(W_QEMPTY + ws));
                 t0 += nt;
+                cur[0] = then[0], cur[1] = then[1];
             }
             if (!ok) note_timeout(a.status);
         }
@@ -901,15 +904,15 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         const f32x2 nm2 = pack2(nm, nm);
                         sum2 = pack2(0.f, 0.f);
                         mx = -INFINITY;
-                        uint32_t sr[2][CW];
-                        tmem_ldw(s_addr, sr[0]);
+                        uint32_t sr[2][16];
+                        tmem_ld16(s_addr, sr[0]);
 #pragma unroll
-                        for (int c = 0; c < 128 / CW; ++c) {
+                        for (int c = 0; c < 8; ++c) {
                             tmem_ld_wait(sr[c & 1]);
-                            if (c < 128 / CW - 1) tmem_ldw(s_addr + (c + 1) * CW, sr[(c + 1) & 1]);
+                            if (c < 8 - 1) tmem_ld16(s_addr + (c + 1) * 16, sr[(c + 1) & 1]);
 #pragma unroll
-                            for (int g = 0; g < CW / 8; ++g) {
-                                const int col = c * CW + g * 8;
+                            for (int g = 0; g < 2; ++g) {
+                                const int col = c * 16 + g * 8;
                                 f32x2 y4[4];
                                 scores8(at_edge, &sr[c & 1][8 * g], col, y4);
                                 const float4 va = *reinterpret_cast<const float4*>(sv + col), vb = *reinterpret_cast<const float4*>(sv + col + 4);
