@@ -575,6 +575,8 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 // 32 scores.
 // The pairs of tiles are taken from a counter, long rows first, by the thread that starts the loads, which runs ahead
 // into the next pair while the last one is finished.
+// (8192 tokens causal, 32/8 heads, D 128: 540 us, 1.02 PFLOP/s; with prefill_attention.cu's shape 622.  Two score blocks of
+// 64 positions per query tile, Q.K^T a tile ahead: 592; halves of 64 with an issuing thread for each query tile: 585.)
 constexpr int kWideThreads = 12 * 32;    // 2 x 4 softmax warps, loads, MMA, and two that fill their warpgroup
 // Registers per thread: 168 at launch; the warpgroup of loads and MMA hands most of its own to the softmax warpgroups
 // (2 * 128 * 224 + 128 * 56 = 384 * 168).
@@ -839,10 +841,11 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             const f32x2 qs2 = pack2(qscale, qscale);
             const int visible = a.causal ? min(job.len, tok + 1) : job.len;             // positions that this row sees
             const int all_visible = a.causal ? first_tok + 1 : job.len;                 // that every row of the tile sees
+            const int any_visible = a.causal ? min(job.len, first_tok + a.tokens) : job.len;   // that some row of it sees
             // the power of two that brings the largest value scale of the sequence to [2^6, 2^7), as an addend of the
             // exponent: it cancels against the sum of the probabilities
             float most = 0.f;
-            const int top_slots = ((a.causal ? min(job.len, first_tok + a.tokens) : job.len) + KT - 1) / KT;
+            const int top_slots = (any_visible + KT - 1) / KT;
             for (int j = lane; j < top_slots && mine > 0; j += 32) most = fmaxf(most, a.top[(long long)job.hk * a.slots + job.kv_slot + j]);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
@@ -863,6 +866,7 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     const float* sv = sk + kWideKT;
                     const int lim = visible - j * kWideKT;               // columns of this tile that the row sees
                     const bool edge = (j + 1) * kWideKT > all_visible;   // (the same for the whole tile)
+                    const int tile_lim = any_visible - j * kWideKT;      // columns that some row of the tile sees
                     // y = (q.k) * sK for 8 columns; columns the row does not see are removed, whatever was there
                     auto scores8 = [&](auto at_edge, const uint32_t* sr8, int c, f32x2* y4) {
                         const float4 ka = *reinterpret_cast<const float4*>(sk + c), kb = *reinterpret_cast<const float4*>(sk + c + 4);
@@ -900,16 +904,17 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     uint32_t P[64];
                     f32x2 sum2;
                     float mx;
-                    auto pass = [&](auto at_edge) {
+                    auto pass = [&](auto at_edge, auto chunks) {         // of 16 columns; the others have no probability
+                        constexpr int CHUNKS = decltype(chunks)::value;
                         const f32x2 nm2 = pack2(nm, nm);
                         sum2 = pack2(0.f, 0.f);
                         mx = -INFINITY;
                         uint32_t sr[2][16];
                         tmem_ld16(s_addr, sr[0]);
 #pragma unroll
-                        for (int c = 0; c < 8; ++c) {
+                        for (int c = 0; c < CHUNKS; ++c) {
                             tmem_ld_wait(sr[c & 1]);
-                            if (c < 8 - 1) tmem_ld16(s_addr + (c + 1) * 16, sr[(c + 1) & 1]);
+                            if (c < CHUNKS - 1) tmem_ld16(s_addr + (c + 1) * 16, sr[(c + 1) & 1]);
 #pragma unroll
                             for (int g = 0; g < 2; ++g) {
                                 const int col = c * 16 + g * 8;
@@ -928,10 +933,16 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                                 P[col / 2 + 2] = pack_h2(s2.x, s2.y), P[col / 2 + 3] = pack_h2(s3.x, s3.y);
                             }
                         }
+#pragma unroll
+                        for (int i = CHUNKS * 8; i < 64; ++i) P[i] = 0u;
                     };
                     for (;;) {
-                        if (edge) pass(std::true_type{});
-                        else pass(std::false_type{});
+                        // a last tile that no row sees the second half of costs half (sixteen prompts up to 2048, 32/8 heads:
+                        // 304 -> 295 us; at head_dim 64 the third form does not fit the registers: 482 -> 507 us for eight
+                        // sequences of 4096, 8 heads)
+                        if (!edge) pass(std::false_type{}, std::integral_constant<int, 8>{});
+                        else if (D == 64 || tile_lim > 64) pass(std::true_type{}, std::integral_constant<int, 8>{});
+                        else pass(std::true_type{}, std::integral_constant<int, 4>{});
                         const bool ahead = mx > lift + kLazyStep;
                         if (!__any_sync(0xffffffffu, ahead)) break;
                         // the reference moves to this tile's maximum, and the tile is done again; P.V of the tile before
