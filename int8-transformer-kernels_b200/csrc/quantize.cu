@@ -339,37 +339,44 @@ __global__ void dequant_tensor_kernel(const int8_t* __restrict__ q, __half* __re
 
 // out[r][c] = fp16(q[r][c] * scale[r]) (+ residual[r][c], added in fp32): the inverse step after the
 // INT8 MLP, which the eager path spells as .float() * scale -> .half() (+ the residual add).
+// A thread takes 8 elements at a time (an 8-byte load, one 16-byte store: a warp writes 512 contiguous bytes) and has
+// four such vectors in flight; the row of a vector by a division of the narrowest type that holds the index (I).
+constexpr int kDequantUnroll = 4;
+template <typename I>
 __global__ void __launch_bounds__(256)
 dequant_rows_kernel(const int8_t* __restrict__ q, const float* __restrict__ scales,
-                    const __half* __restrict__ residual, __half* __restrict__ out, long long vecs, int vecs_per_row) {
+                    const __half* __restrict__ residual, __half* __restrict__ out, I vecs, I vecs_per_row) {
     pdl_wait();
     pdl_launch_dependents();
-    for (long long v = (long long)blockIdx.x * blockDim.x + threadIdx.x; v < vecs;
-         v += (long long)gridDim.x * blockDim.x) {
-        const float sc = scales[v / vecs_per_row];
-        const uint4 w = *reinterpret_cast<const uint4*>(q + v * 16);
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-        uint4 r0 = make_uint4(0u, 0u, 0u, 0u), r1 = r0;
-        if (residual) {
-            r0 = *reinterpret_cast<const uint4*>(residual + v * 16);
-            r1 = *reinterpret_cast<const uint4*>(residual + v * 16 + 8);
+    const I first = (I)blockIdx.x * (kDequantUnroll * 256) + threadIdx.x;
+    float sc[kDequantUnroll];
+    uint2 w[kDequantUnroll];
+    uint4 r[kDequantUnroll];
+#pragma unroll
+    for (int u = 0; u < kDequantUnroll; ++u) {
+        const I v = first + u * 256;
+        sc[u] = 0.f, w[u] = make_uint2(0u, 0u), r[u] = make_uint4(0u, 0u, 0u, 0u);
+        if (v < vecs) {
+            sc[u] = scales[v / vecs_per_row];
+            w[u] = *reinterpret_cast<const uint2*>(q + (long long)v * 8);
+            if (residual) r[u] = *reinterpret_cast<const uint4*>(residual + (long long)v * 8);
         }
-        const __half2* rh0 = reinterpret_cast<const __half2*>(&r0);
-        const __half2* rh1 = reinterpret_cast<const __half2*>(&r1);
-        uint32_t o[8];
+    }
+#pragma unroll
+    for (int u = 0; u < kDequantUnroll; ++u) {
+        const I v = first + u * 256;
+        if (v >= vecs) break;
+        const __half2* rh = reinterpret_cast<const __half2*>(&r[u]);
+        uint32_t o[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-            const int b0 = (int)(int8_t)(ww[k] & 0xff), b1 = (int)(int8_t)((ww[k] >> 8) & 0xff);
-            const int b2 = (int)(int8_t)((ww[k] >> 16) & 0xff), b3 = (int)(int8_t)(ww[k] >> 24);
-            const float2 ra = __half22float2(k < 2 ? rh0[2 * k] : rh1[2 * k - 4]);
-            const float2 rb = __half22float2(k < 2 ? rh0[2 * k + 1] : rh1[2 * k - 3]);
-            const __half2 ha = __floats2half2_rn(fmaf((float)b0, sc, ra.x), fmaf((float)b1, sc, ra.y));
-            const __half2 hb = __floats2half2_rn(fmaf((float)b2, sc, rb.x), fmaf((float)b3, sc, rb.y));
-            o[2 * k] = *reinterpret_cast<const uint32_t*>(&ha);
-            o[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&hb);
+            const uint32_t ww = k < 2 ? w[u].x : w[u].y;
+            const int b0 = (int)(int8_t)(ww >> (16 * (k & 1))), b1 = (int)(int8_t)(ww >> (16 * (k & 1) + 8));
+            const float2 ra = __half22float2(rh[k]);
+            const __half2 ha = __floats2half2_rn(fmaf((float)b0, sc[u], ra.x), fmaf((float)b1, sc[u], ra.y));
+            o[k] = *reinterpret_cast<const uint32_t*>(&ha);
         }
-        *reinterpret_cast<uint4*>(out + v * 16) = make_uint4(o[0], o[1], o[2], o[3]);
-        *reinterpret_cast<uint4*>(out + v * 16 + 8) = make_uint4(o[4], o[5], o[6], o[7]);
+        *reinterpret_cast<uint4*>(out + (long long)v * 8) = make_uint4(o[0], o[1], o[2], o[3]);
     }
 }
 
@@ -409,12 +416,16 @@ extern "C" int i8tk_dequantize_per_token_f16(const int8_t* q, const float* scale
     I8TK_REQUIRE(q && scales && out_f16, I8TK_ERR_INVALID_ARGUMENT, "null pointer argument");
     I8TK_REQUIRE(aligned_to(q, 16) && aligned_to(out_f16, 16) && (!residual_f16 || aligned_to(residual_f16, 16)),
                  I8TK_ERR_ALIGNMENT, "q, out and residual must be 16-byte aligned");
-    const long long vecs = rows * (cols / 16);
-    long long blocks = (vecs + 255) / 256;
-    if (blocks > 148ll * 16) blocks = 148ll * 16;
-    I8TK_CUDA(launch_after(dequant_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, static_cast<cudaStream_t>(stream),
-                           q, scales, static_cast<const __half*>(residual_f16), static_cast<__half*>(out_f16), vecs,
-                           cols / 16));
+    const long long vecs = rows * (cols / 8), blocks = (vecs + kDequantUnroll * 256 - 1) / (kDequantUnroll * 256);
+    I8TK_REQUIRE(blocks < (1ll << 31), I8TK_ERR_UNSUPPORTED, "too many elements");
+    const dim3 grid((unsigned)blocks), block(256);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const __half* res = static_cast<const __half*>(residual_f16);
+    __half* out = static_cast<__half*>(out_f16);
+    if (vecs < (1ll << 31))
+        I8TK_CUDA(launch_after(dequant_rows_kernel<uint32_t>, grid, block, 0, st, q, scales, res, out, vecs, cols / 8));
+    else
+        I8TK_CUDA(launch_after(dequant_rows_kernel<long long>, grid, block, 0, st, q, scales, res, out, vecs, cols / 8));
     return I8TK_OK;
 }
 
