@@ -72,8 +72,9 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
-template <typename T, int D, bool QUANT>
-__global__ void __launch_bounds__(kThreads)
+// ROT: 0 no rotation, 1 half-split pairs, 2 interleaved pairs.
+template <typename T, int D, bool QUANT, int ROT>
+__global__ void __launch_bounds__(kThreads, 8)
 qk_norm_rope_kernel(const QkArgs a) {
     constexpr int LPR = D / 8;                       // lanes per row
     constexpr int GROUPS = 32 / LPR;                 // rows a warp holds side by side
@@ -90,47 +91,95 @@ qk_norm_rope_kernel(const QkArgs a) {
     const int kind = unit < a.q_units ? 0 : unit < a.q_units + a.k_units ? 1 : 2;
     const int head0 = kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads;
     const int count = kind == 0 ? a.heads : a.kv_heads;
-    const int first = (unit - (kind == 0 ? 0 : kind == 1 ? a.q_units : a.q_units + a.k_units)) * PER + lane / LPR;
+    const int unit0 = (unit - (kind == 0 ? 0 : kind == 1 ? a.q_units : a.q_units + a.k_units)) * PER;    // first head of the warp
+    const int left = count - unit0 - lane / LPR;     // heads from this group's first one on
     const int total = a.heads + a.kv_heads * (QUANT ? 2 : 1);
+    const int first = head0 + unit0 + lane / LPR;    // this group's first head of the token
 
-    const T* row = static_cast<const T*>(a.qkv) + t * a.row_stride + (long long)head0 * D + d0;
+    const T* row = static_cast<const T*>(a.qkv) + t * a.row_stride + (first * D + d0);
     uint4 raw[kRows];
 #pragma unroll
-    for (int i = 0; i < kRows; ++i) {
-        const int h = first + i * GROUPS;
-        raw[i] = h < count ? *reinterpret_cast<const uint4*>(row + (long long)h * D) : make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < kRows; ++i)
+        raw[i] = i * GROUPS < left ? *reinterpret_cast<const uint4*>(row + i * GROUPS * D) : make_uint4(0u, 0u, 0u, 0u);
+
+    const long long at = t * total + first;
+    T* out = static_cast<T*>(a.out) + at * D + d0;
+    int8_t* codes = a.codes + at * D + d0;
+    float* scales = a.scales + at;
+    const f32x2 magic = pack2(12582912.f, 12582912.f), minus = pack2(-1.f, -1.f);
+    auto store_codes = [&](int i, const f32x2* q, float scale) {
+        if (i * GROUPS < left) {
+            const uint32_t b0 = prmt(__float_as_uint(q[0].x), __float_as_uint(q[0].y), 0x0040), b1 = prmt(__float_as_uint(q[1].x), __float_as_uint(q[1].y), 0x0040);
+            const uint32_t b2 = prmt(__float_as_uint(q[2].x), __float_as_uint(q[2].y), 0x0040), b3 = prmt(__float_as_uint(q[3].x), __float_as_uint(q[3].y), 0x0040);
+            *reinterpret_cast<uint2*>(codes + i * GROUPS * D) = make_uint2(prmt(b0, b1, 0x5410), prmt(b2, b3, 0x5410));
+            if (sub == 0) scales[i * GROUPS] = scale;
+        }
+    };
+    auto row_max = [&](const f32x2* u) {
+        float mx = max3(max3(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y),
+                        max3(fabsf(u[2].x), fabsf(u[2].y), fmaxf(fabsf(u[3].x), fabsf(u[3].y))));
+#pragma unroll
+        for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+        return mx;
+    };
+
+    if (QUANT && (kind == 2 || (ROT == 0 && a.q_weight == nullptr))) {
+        // rows that are only quantised get exactly the per-token quantiser: a quotient next to a tie is divided
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            if (unit0 + i * GROUPS >= count) break;  // the whole warp is past the last head
+            const f32x2 u[4] = {widen(tag, raw[i].x), widen(tag, raw[i].y), widen(tag, raw[i].z), widen(tag, raw[i].w)};
+            const float scale = div127(fmaxf(row_max(u), 1e-8f)), inv = rcp_approx(scale);
+            const f32x2 inv2 = pack2(inv, inv);
+            f32x2 q[4];
+            float off = 0.f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                q[k] = fma2(u[k], inv2, magic);
+                const f32x2 d = fma2(u[k], inv2, fma2(q[k], minus, magic));      // the quotient less its rounding
+                off = max3(off, fabsf(d.x), fabsf(d.y));
+            }
+            if (off > 0.4999f) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) q[k] = pack2(rintf(__fdiv_rn(u[k].x, scale)) + 12582912.f, rintf(__fdiv_rn(u[k].y, scale)) + 12582912.f);
+            }
+            store_codes(i, q, scale);
+            if (kind == 1 && a.k_out != nullptr && i * GROUPS < left)
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (t * a.kv_heads + (first - head0) + i * GROUPS) * D + d0) = raw[i];
+        }
+        return;
     }
 
     // ---- what the rows share: w c and w' s of this lane's channels ----
     f32x2 wc[4], ws[4];
     const int half_r = a.R >> 1;
-    const bool norm = kind < 2 && a.q_weight != nullptr;
-    const bool turn = kind < 2 && a.positions != nullptr && d0 < a.R;   // R is a multiple of 16: all of a lane's channels or none
+    const bool norm = a.q_weight != nullptr;
+    const bool turn = ROT != 0 && d0 < a.R;          // R is a multiple of 16: all of a lane's channels or none
     const int partner = d0 < half_r ? sub + half_r / 8 : sub - half_r / 8;     // lane of the half-split partner
-    const int from = lane - sub + (turn && !a.interleaved ? partner : sub);
+    const int from = lane - sub + (ROT == 1 && turn ? partner : sub);
     bool known = true;                               // a position without a table row shows in the result
-    if (kind < 2) {
+    {
         const float* weight = kind == 0 ? a.q_weight : a.k_weight;
         float w[8], wp[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[k] = wp[k] = 1.0f;
         if (norm) {
-            const float* at = weight + d0;
-            const float* other = weight + (turn && !a.interleaved ? partner * 8 : d0);
+            const float* own = weight + d0;
+            const float* other = weight + (ROT == 1 && turn ? partner * 8 : d0);
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-                const float4 x = *reinterpret_cast<const float4*>(at + 4 * k), y = *reinterpret_cast<const float4*>(other + 4 * k);
+                const float4 x = *reinterpret_cast<const float4*>(own + 4 * k), y = *reinterpret_cast<const float4*>(other + 4 * k);
                 w[4 * k] = x.x, w[4 * k + 1] = x.y, w[4 * k + 2] = x.z, w[4 * k + 3] = x.w;
                 wp[4 * k] = y.x, wp[4 * k + 1] = y.y, wp[4 * k + 2] = y.z, wp[4 * k + 3] = y.w;
             }
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) wc[k] = pack2(w[2 * k], w[2 * k + 1]), ws[k] = pack2(0.f, 0.f);
-        if (a.positions != nullptr) {
+        if constexpr (ROT != 0) {
             const int pos = a.positions[t];
             known = pos >= 0 && pos < a.rope_rows;
             const float* tab = a.rope + (long long)(known ? pos : 0) * a.R;
-            if (turn && a.interleaved) {             // four pairs of this lane: the partner is the other half of a word
+            if (ROT == 2 && turn) {                  // four pairs of this lane: the partner is the other half of a word
                 const float4 c = *reinterpret_cast<const float4*>(tab + (d0 >> 1)), s = *reinterpret_cast<const float4*>(tab + half_r + (d0 >> 1));
                 const float cs[4] = {c.x, c.y, c.z, c.w}, sn[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
@@ -158,86 +207,59 @@ qk_norm_rope_kernel(const QkArgs a) {
 
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-        const int h = first + i * GROUPS;
-        if (h - lane / LPR >= count) break;          // the whole warp is past the last head
+        if (unit0 + i * GROUPS >= count) break;      // the whole warp is past the last head
         const uint32_t x4[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
         f32x2 u[4];
-        float r = 1.0f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) u[k] = widen(tag, x4[k]);
-        if (norm) {
-            f32x2 sq = mul2(u[0], u[0]);
+        f32x2 sq = mul2(u[0], u[0]);
 #pragma unroll
-            for (int k = 1; k < 4; ++k) sq = fma2(u[k], u[k], sq);
-            float ss = sq.x + sq.y;
+        for (int k = 1; k < 4; ++k) sq = fma2(u[k], u[k], sq);
+        float ss = sq.x + sq.y;
 #pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            r = rsqrtf(ss * (1.0f / D) + a.eps);
-        }
-        if (kind < 2) {
+        for (int o = LPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        const float r = norm ? rsqrtf(ss * (1.0f / D) + a.eps) : 1.0f;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], wc[k]);
+        if constexpr (ROT != 0) {
             uint32_t z4[4];
-            if (a.interleaved) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) z4[k] = prmt(x4[k], 0u, 0x1032u);
-            } else {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) z4[k] = __shfl_sync(0xffffffffu, x4[k], from);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], wc[k]);
+            for (int k = 0; k < 4; ++k) z4[k] = ROT == 2 ? prmt(x4[k], 0u, 0x1032u) : __shfl_sync(0xffffffffu, x4[k], from);
             if (turn) {                              // (a lane outside the rotated channels must not see 0 * infinity)
 #pragma unroll
                 for (int k = 0; k < 4; ++k) u[k] = fma2(widen(tag, z4[k]), ws[k], u[k]);
             }
         }
+        const f32x2 r2 = pack2(r, r);
         if constexpr (!QUANT) {
-            const f32x2 r2 = pack2(r, r);
 #pragma unroll
             for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], r2);
-            if (h < count)
-                *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (t * total + head0 + h) * D + d0) =
+            if (i * GROUPS < left)
+                *reinterpret_cast<uint4*>(out + i * GROUPS * D) =
                     make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
         } else {
-            float mx = max3(max3(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y), max3(fabsf(u[2].x), fabsf(u[2].y), fmaxf(fabsf(u[3].x), fabsf(u[3].y))));
-#pragma unroll
-            for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float scale = known ? div127(fmaxf(mx * r, 1e-8f)) : __int_as_float(0x7fc00000);
+            const float scale = known ? div127(fmaxf(row_max(u) * r, 1e-8f)) : __int_as_float(0x7fc00000);
             const float inv = rcp_approx(scale) * r;
-            const f32x2 inv2 = pack2(inv, inv), magic = pack2(12582912.f, 12582912.f);
+            const f32x2 inv2 = pack2(inv, inv);
             f32x2 q[4];
 #pragma unroll
             for (int k = 0; k < 4; ++k) q[k] = fma2(u[k], inv2, magic);
-            if (kind == 2 || (a.q_weight == nullptr && a.positions == nullptr)) {
-                // rows that are only quantised get exactly the per-token quantiser: a quotient next to a tie is divided
-                const f32x2 nm = pack2(-12582912.f, -12582912.f);
-                float off = 0.f;
+            store_codes(i, q, scale);
+            if (kind == 1 && a.k_out != nullptr && i * GROUPS < left) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const f32x2 n = add2(q[k], nm), d = fma2(u[k], inv2, pack2(-n.x, -n.y));
-                    off = max3(off, fabsf(d.x), fabsf(d.y));
-                }
-                if (off > 0.4999f) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        q[k] = pack2(rintf(__fdiv_rn(u[k].x, scale)) + 12582912.f, rintf(__fdiv_rn(u[k].y, scale)) + 12582912.f);
-                }
-            }
-            if (h < count) {
-                const long long at = t * total + head0 + h;
-                const uint32_t b0 = prmt(__float_as_uint(q[0].x), __float_as_uint(q[0].y), 0x0040), b1 = prmt(__float_as_uint(q[1].x), __float_as_uint(q[1].y), 0x0040);
-                const uint32_t b2 = prmt(__float_as_uint(q[2].x), __float_as_uint(q[2].y), 0x0040), b3 = prmt(__float_as_uint(q[3].x), __float_as_uint(q[3].y), 0x0040);
-                *reinterpret_cast<uint2*>(a.codes + at * D + d0) = make_uint2(prmt(b0, b1, 0x5410), prmt(b2, b3, 0x5410));
-                if (sub == 0) a.scales[at] = scale;
-                if (kind == 1 && a.k_out != nullptr) {
-                    const f32x2 r2 = pack2(r, r);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], r2);
-                    *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (t * a.kv_heads + h) * D + d0) =
-                        make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
-                }
+                for (int k = 0; k < 4; ++k) u[k] = mul2(u[k], r2);
+                *reinterpret_cast<uint4*>(static_cast<T*>(a.k_out) + (t * a.kv_heads + (first - head0) + i * GROUPS) * D + d0) =
+                    make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
             }
         }
     }
+}
+
+template <typename T, int D, bool QUANT>
+cudaError_t launch_rot(const QkArgs& a, dim3 grid, cudaStream_t st) {
+    if (a.positions == nullptr) return launch_after(qk_norm_rope_kernel<T, D, QUANT, 0>, grid, dim3(kThreads), 0, st, a);
+    if (!a.interleaved) return launch_after(qk_norm_rope_kernel<T, D, QUANT, 1>, grid, dim3(kThreads), 0, st, a);
+    return launch_after(qk_norm_rope_kernel<T, D, QUANT, 2>, grid, dim3(kThreads), 0, st, a);
 }
 
 template <typename T, bool QUANT>
@@ -248,10 +270,8 @@ int launch_qk(QkArgs a, int D, cudaStream_t st) {
     a.units = a.q_units + a.k_units * (QUANT ? 2 : 1);
     const long long blocks = (a.tokens + kThreads / 32 - 1) / (kThreads / 32) * a.units;
     I8TK_REQUIRE(blocks < (1ll << 31), I8TK_ERR_UNSUPPORTED, "too many tokens");
-    const dim3 grid((unsigned)blocks), block(kThreads);
-    if (D == 64) I8TK_CUDA(launch_after(qk_norm_rope_kernel<T, 64, QUANT>, grid, block, 0, st, a));
-    else if (D == 128) I8TK_CUDA(launch_after(qk_norm_rope_kernel<T, 128, QUANT>, grid, block, 0, st, a));
-    else I8TK_CUDA(launch_after(qk_norm_rope_kernel<T, 256, QUANT>, grid, block, 0, st, a));
+    const dim3 grid((unsigned)blocks);
+    I8TK_CUDA((D == 64 ? launch_rot<T, 64, QUANT>(a, grid, st) : D == 128 ? launch_rot<T, 128, QUANT>(a, grid, st) : launch_rot<T, 256, QUANT>(a, grid, st)));
     return I8TK_OK;
 }
 
