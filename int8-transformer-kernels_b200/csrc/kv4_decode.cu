@@ -23,9 +23,9 @@
 //   for one octet per lane instead of for W of which only one has heads in the lane.  A copy keeps a maximum and sums of
 //   its own, as a row apart, and the copies are merged with the warps' rows.
 //
-// The tiles (128 positions) of all (request, key head) rows, in that order, are one sequence, cut into equal runs for
+// The tiles (128 positions, 256 at head_dim 64) of all (request, key head) rows, in that order, are one sequence, cut into equal runs for
 // the CTAs from the lengths on the device: a short request costs what it reads.  Every CTA adds the lengths up itself
-// (they are a few hundred words), so nothing runs ahead of the scan.  A CTA is four warps, 32 positions of a tile each,
+// (they are a few hundred words), so nothing runs ahead of the scan.  A CTA is four warps, a quarter of a tile each,
 // which meet only where a row ends; in turn they start the bulk copies of the next tile, one copy per page and head.
 // There is no warp for the copies alone: the unpacking is bound by the instructions the SM can issue, and four CTAs of
 // four 128-register warps are all it holds (with a fifth warp it held three).  The page size is a template parameter,
@@ -39,8 +39,10 @@
 namespace i8tk {
 namespace {
 
-constexpr int kTile = 128;                  // positions
-constexpr int kWarps = 4;                   // 32 positions each
+// Positions of a tile: about 18 KB of the cache.  A warp takes a quarter, 32 positions at a time.  (128 positions at
+// head_dim 64 too: 16 requests of 16384, 12/12 heads, 60.7 us against 55.4.)
+__host__ __device__ constexpr int tile_of(int D) { return D == 64 ? 256 : 128; }
+constexpr int kWarps = 4;
 constexpr int kScanThreads = kWarps * 32;
 // P = p * s has to stay an fp16 number (below 2^16) and should use its range: a row's reference lies kTop log2 units
 // below its largest score times the largest scale met so far, and moves when a product would run kSlack above that.
@@ -51,7 +53,7 @@ constexpr float kNoReference = 1e30f;       // negative reference of a row that 
 template <int D, int NT, int W>             // NT: blocks of 8 query heads per key head; W: copies of the heads in a block
 struct Kv4Cfg {
     static constexpr int G = D / 64;
-    static constexpr int TILE_BYTES = kTile * (D + D / 8);
+    static constexpr int TILE = tile_of(D), TILE_BYTES = TILE * (D + D / 8);
     // Two stages: a third (32 requests, up to 32768 positions, 32/8 heads, D 128: 127 us a call waited for, against 134)
     // fills the SM's shared memory, and a call that follows at once loses more (153 us against 122).
     static constexpr int STAGES = 2;
@@ -90,7 +92,8 @@ __device__ __forceinline__ void note(const Kv4Args& a, uint32_t what, uint32_t c
 __device__ __forceinline__ int row_len(const Kv4Args& a, int b) {
     return min(max(__ldg(a.lens + b), 0), a.max_len);
 }
-__device__ __forceinline__ int row_tiles(const Kv4Args& a, int b) { return (row_len(a, b) + kTile - 1) / kTile; }
+template <int D>
+__device__ __forceinline__ int row_tiles(const Kv4Args& a, int b) { return (row_len(a, b) + tile_of(D) - 1) / tile_of(D); }
 // The first n CTAs have a run each, none of them empty: n is the grid or, with fewer tiles than that, their number.
 // First tile of CTA c's run, and the CTA that a tile belongs to.
 __device__ __forceinline__ int runs_of(long long total, int ctas) { return total < ctas ? (int)total : ctas; }
@@ -134,18 +137,20 @@ __device__ __forceinline__ float2 pair_of(uint32_t w) { return __half22float2(*r
 struct Row {
     int b, h, len, tiles;
 };
+template <int D>
 __device__ __forceinline__ void load_row(const Kv4Args& a, Row& r) {
     r.len = row_len(a, r.b);
-    r.tiles = (r.len + kTile - 1) / kTile;
+    r.tiles = (r.len + tile_of(D) - 1) / tile_of(D);
 }
 // the next row that has tiles; called only while tiles remain, the bound on b (and the length it then gives) is for
 // lengths that changed under the kernel
+template <int D>
 __device__ __forceinline__ void next_row(const Kv4Args& a, Row& r) {
     if (++r.h < a.kv_heads) return;
     r.h = 0;
     while (r.b + 1 < a.B) {
         ++r.b;
-        load_row(a, r);
+        load_row<D>(a, r);
         if (r.tiles > 0) return;
     }
     r.tiles = 1 << 30, r.len = 0;
@@ -180,7 +185,7 @@ kv4_scan_kernel(const Kv4Args a) {
     const int per = (a.B + kScanThreads - 1) / kScanThreads;
     const int lo = min(a.B, (int)threadIdx.x * per), hi = min(a.B, lo + per);
     int mine = 0;
-    for (int b = lo; b < hi; ++b) mine += row_tiles(a, b);
+    for (int b = lo; b < hi; ++b) mine += row_tiles<D>(a, b);
     int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -203,7 +208,7 @@ kv4_scan_kernel(const Kv4Args a) {
     if (mine > 0 && (long long)before * a.kv_heads <= first && first < (long long)(before + mine) * a.kv_heads) {
         int at = before;
         for (int b = lo; b < hi; ++b) {
-            const int n = row_tiles(a, b);
+            const int n = row_tiles<D>(a, b);
             if (first < (long long)(at + n) * a.kv_heads) {
                 s_start[0] = b, s_start[1] = at;
                 break;
@@ -215,7 +220,7 @@ kv4_scan_kernel(const Kv4Args a) {
         int at = before;
         for (int b = lo; b < hi; ++b) {
             a.prefix[b] = at;
-            at += row_tiles(a, b);
+            at += row_tiles<D>(a, b);
         }
         if (threadIdx.x == 0) a.prefix[a.B] = sum;
     }
@@ -224,7 +229,7 @@ kv4_scan_kernel(const Kv4Args a) {
     if (run == 0) return;
     Row cur;
     cur.b = s_start[0];
-    load_row(a, cur);
+    load_row<D>(a, cur);
     int tile;                                // of the row
     {
         const long long in = first - (long long)s_start[1] * a.kv_heads;
@@ -232,7 +237,7 @@ kv4_scan_kernel(const Kv4Args a) {
         tile = (int)(in - (long long)cur.h * cur.tiles);
     }
     static_assert(kv4_block_bytes(PAGE, D) % D == 0 && Cfg::TILE_BYTES % D == 0, "rows pair up by one address bit");
-    constexpr int BLOCK = kv4_block_bytes(PAGE, D), PAGES = kTile / PAGE;      // pages of a tile: 1 to 8, a lane each
+    constexpr int BLOCK = kv4_block_bytes(PAGE, D), PAGES = Cfg::TILE / PAGE;  // pages of a tile: 1 to 16, a lane each
 
     // ---- copies: tile i of the run is brought by warp i % 4, a lane per page, STAGES - 1 tiles ahead ----
     auto look_up = [&](const Row& r, int t) {
@@ -243,16 +248,16 @@ kv4_scan_kernel(const Kv4Args a) {
     auto find = [&](Row& r, int& t) {
         while (t >= r.tiles) {
             t -= r.tiles;
-            next_row(a, r);
+            next_row<D>(a, r);
         }
     };
     auto issue = [&](const Row& r, int t, int id, int s) {       // tile t of row r, whose page ids the lanes hold, into stage s
-        const int left = max(r.len - t * kTile, 0);
+        const int left = max(r.len - t * Cfg::TILE, 0);
         if ((unsigned)id >= (unsigned)a.num_pages) {                           // never followed
             id = 0;
             note(a, kNotedBadIndex, 1u);
         }
-        if (lane == 0) mbar_expect_tx(full(s), (left >= kTile ? PAGES : (left + PAGE - 1) / PAGE) * BLOCK);
+        if (lane == 0) mbar_expect_tx(full(s), (left >= Cfg::TILE ? PAGES : (left + PAGE - 1) / PAGE) * BLOCK);
         __syncwarp();
         if (lane < PAGES && lane * PAGE < left)
             bulk_g2s(base + s * Cfg::TILE_BYTES + lane * BLOCK, a.pool + ((long long)id * a.kv_heads + r.h) * BLOCK, BLOCK, full(s));
@@ -336,12 +341,13 @@ kv4_scan_kernel(const Kv4Args a) {
     }
     // this thread's rows: keys at row `row` of its 16, values at row vrow, both of the warp's first 16 positions
     constexpr int U = PAGE == 16 ? BLOCK : 16 * (D / 2), U_PAIRS = PAGE == 16 ? BLOCK : 16 * G * 4;     // to the next 16
-    const int p0 = warp * 32, in_page = p0 % PAGE;
+    const int p0 = warp * (Cfg::TILE / kWarps), in_page = p0 % PAGE;
     const int warp_block = p0 / PAGE * BLOCK;
     int k_at = warp_block + (in_page + row) * (D / 2) + tig * (D / 8);
     int pair_at = warp_block + PAGE * D + (in_page + row + 8 * my_e) * (G * 4) + my_u * U_PAIRS;
     int v_at = warp_block + PAGE * (D / 2) + (in_page + vrow) * (D / 2) + gid * (G * 4);
-    constexpr int PAIRS = PAGE * G * 4;                     // from the keys' pairs to the values'
+    constexpr int PAIRS = PAGE * G * 4;                      // from the keys' pairs to the values'
+    constexpr int SUB = PAGE >= 64 ? 32 * (D / 2) : 32 / PAGE * BLOCK, SUB_PAIRS = PAGE >= 64 ? 32 * G * 4 : 32 / PAGE * BLOCK;    // to the next 32
     auto next_stage = [&]() {
         const bool wrap = s == Cfg::STAGES - 1;
         const int to = wrap ? -(Cfg::STAGES - 1) * Cfg::TILE_BYTES : Cfg::TILE_BYTES;
@@ -353,9 +359,9 @@ kv4_scan_kernel(const Kv4Args a) {
         const int pieces = min(cur.tiles - tile, run - i), seg_first = tile;
         const bool row_ends = tile + pieces == cur.tiles, more = i + pieces < run;
         begin_row();
-        int left = cur.len - tile * kTile - warp * 32;           // positions of this warp's 32 that exist
+        int here = cur.len - tile * Cfg::TILE - p0;              // positions of this warp's quarter that exist
         int ahead_id = 0;                                        // page ids of this warp's next turn in this row
-        for (int k = 0; k < pieces; ++k, ++i, left -= kTile) {
+        for (int k = 0; k < pieces; ++k, ++i, here -= Cfg::TILE) {
             // ---- the tile STAGES - 1 ahead, into the stage the last one was read from ----
             if (((i + Cfg::STAGES - 1) & 3) == warp && i + Cfg::STAGES - 1 < run) {
                 const int o = s == 0 ? Cfg::STAGES - 1 : s - 1;
@@ -380,7 +386,9 @@ kv4_scan_kernel(const Kv4Args a) {
                     if (!__all_sync(0xffffffffu, at_last)) goto late;
                 }
             }
-            if (left > 0) {
+#pragma unroll 1
+            for (int sub = 0, left = here; sub < Cfg::TILE / kWarps / 32 && left > 0; ++sub, left -= 32) {
+                const int ks = k_at + sub * SUB, ps = pair_at + sub * SUB_PAIRS, vs = v_at + sub * SUB;
             // ---- scores of 2 x 16 positions ----
             f32x2 sc[NU][NE][NT];                            // [16 positions][row gid, gid + 8][8 columns]
             uint32_t vp[NU][NE][G];                          // the values' pairs of the same positions
@@ -388,8 +396,8 @@ kv4_scan_kernel(const Kv4Args a) {
             float dot[2][NT][G][4];
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
-                lds_words(smem + k_at + u * U, wa[u]);
-                lds_words(smem + k_at + u * U + 8 * (D / 2), wb[u]);
+                lds_words(smem + ks + u * U, wa[u]);
+                lds_words(smem + ks + u * U + 8 * (D / 2), wb[u]);
             }
 #pragma unroll
             for (int w = 0; w < 2 * G; ++w) {
@@ -412,8 +420,8 @@ kv4_scan_kernel(const Kv4Args a) {
 #pragma unroll
                 for (int e = 0; e < NE; ++e) {
                     uint32_t kp[G];
-                    lds_words(smem + pair_at + u * U_PAIRS + 8 * e * (G * 4), kp);
-                    lds_words(smem + pair_at + u * U_PAIRS + 8 * e * (G * 4) + PAIRS, vp[u][e]);
+                    lds_words(smem + ps + u * U_PAIRS + 8 * e * (G * 4), kp);
+                    lds_words(smem + ps + u * U_PAIRS + 8 * e * (G * 4) + PAIRS, vp[u][e]);
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
                         const float2 sz = pair_of(kp[g]);
@@ -535,10 +543,10 @@ kv4_scan_kernel(const Kv4Args a) {
                         }
                 uint32_t v0[G], v1[G], v2[G], v3[G];
                 // the odd position of the pair: blocks and stages are multiples of two rows
-                lds_words(smem + v_at + u * U, v0);
-                lds_words(smem + (v_at ^ (D / 2)) + u * U, v1);
-                lds_words(smem + v_at + u * U + 8 * (D / 2), v2);
-                lds_words(smem + (v_at ^ (D / 2)) + u * U + 8 * (D / 2), v3);
+                lds_words(smem + vs + u * U, v0);
+                lds_words(smem + (vs ^ (D / 2)) + u * U, v1);
+                lds_words(smem + vs + u * U + 8 * (D / 2), v2);
+                lds_words(smem + (vs ^ (D / 2)) + u * U + 8 * (D / 2), v3);
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
 #pragma unroll
@@ -630,7 +638,7 @@ kv4_scan_kernel(const Kv4Args a) {
         __syncwarp();
         if (lane == 0) mbar_arrive(empty(s));
         next_stage();
-        if (more) next_row(a, cur);
+        if (more) next_row<D>(a, cur);
         tile = 0;
     }
     return;
@@ -723,7 +731,7 @@ int resident_ctas(int group) {
 
 Kv4Layout kv4_layout(int B, int kv_heads, int group, int max_len, int D) {
     Kv4Layout y;
-    const long long tiles = (long long)B * kv_heads * ((max_len + kTile - 1) / kTile);
+    const long long tiles = (long long)B * kv_heads * ((max_len + tile_of(D) - 1) / tile_of(D));
     const long long resident = (long long)sms() * resident_ctas(group);
     y.ctas = (int)(tiles < resident ? tiles : resident);
     y.prefix_off = 256;
@@ -735,7 +743,7 @@ Kv4Layout kv4_layout(int B, int kv_heads, int group, int max_len, int D) {
 
 bool kv4_shape_ok(int B, int heads, int kv_heads, int max_len, int D) {
     return B > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0 && heads / kv_heads <= 16 && max_len > 0 && (D == 64 || D == 128) &&
-           (long long)B * kv_heads * ((max_len + kTile - 1) / kTile) < (1ll << 31) && (long long)B * kv_heads < (1ll << 31);
+           (long long)B * kv_heads * ((max_len + tile_of(D) - 1) / tile_of(D)) < (1ll << 31) && (long long)B * kv_heads < (1ll << 31);
 }
 
 template <int D, int NT, int W, int PAGE>

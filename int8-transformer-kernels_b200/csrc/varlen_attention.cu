@@ -90,7 +90,8 @@ struct Packed {
     __half* out;                 // [T][heads][D]
     float score_scale_log2;
     uint32_t* status;
-    uint32_t* counter;           // work taken so far (head_dim 64 and 128); the pre-pass sets it to zero
+    uint32_t* counter;           // work taken so far beyond a first piece per CTA (head_dim 64 and 128); the pre-pass
+                                 // sets it to zero
 };
 
 // The sequence that owns slot `slot` of n-token slots, its first row and length, and the slot's place in it.  Values of
@@ -100,20 +101,29 @@ struct Seq {
     int whole;                   // length before it is cut to max_len
 };
 __device__ __forceinline__ int cu_at(const int* cu, int i, int T) { return min(max(__ldg(cu + i), 0), T); }
+// A whole warp looks: 32 probes a round, so up to 32 sequences cost one load's latency, up to 1024 two.
 __device__ __forceinline__ Seq find_sequence(const int* cu, int B, int T, int max_len, int slot, int n) {
-    int lo = 0, hi = B - 1;                  // largest b with cu[b] / n + b <= slot
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (cu_at(cu, mid, T) / n + mid <= slot) lo = mid;
-        else hi = mid - 1;
+    const int lane = threadIdx.x & 31;
+    int lo = 0, hi = B - 1;                  // largest b with cu[b] / n + b <= slot, or 0
+    for (;;) {
+        const int step = (hi - lo + 32) >> 5, b = min(lo + lane * step, hi);
+        const int from = cu_at(cu, b, T), to = cu_at(cu, b + 1, T);
+        const unsigned below = __ballot_sync(0xffffffffu, from / n + b <= slot);
+        // the last probe of the unbroken run from lane 0 on (a damaged table may break it)
+        const int run = below == 0xffffffffu ? 32 : __ffs((int)~below) - 1, at = max(run - 1, 0);
+        if (step == 1) {
+            Seq s;
+            const int found = min(lo + at, hi);
+            s.start = __shfl_sync(0xffffffffu, from, at);
+            s.whole = max(__shfl_sync(0xffffffffu, to, at) - s.start, 0);
+            s.len = min(s.whole, max_len);
+            s.first_slot = s.start / n + found;
+            s.local = slot - s.first_slot;
+            return s;
+        }
+        lo = min(lo + at * step, hi);
+        hi = min(lo + step - 1, hi);
     }
-    Seq s;
-    s.start = cu_at(cu, lo, T);
-    s.whole = max(cu_at(cu, lo + 1, T) - s.start, 0);
-    s.len = min(s.whole, max_len);
-    s.first_slot = s.start / n + lo;
-    s.local = slot - s.first_slot;
-    return s;
 }
 
 __device__ __forceinline__ uint32_t pack_h2(float a, float b) {
@@ -674,67 +684,73 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
-        // ================= work and loads =================
-        if (lane == 0) {
-            const int slots = a.T / two + a.B, items = slots * a.kv_heads;
-            bool ok = true;
-            int t = 0;                                       // key tiles loaded so far
-            int next = (int)atomicAdd(a.counter, 1u);
-            for (int w = 0; ok; ++w) {
-                WideWork x;
-                x.nt_a = -1;
-                for (;;) {                                   // to a slot that has rows
-                    const int item = next;
-                    if (item >= items) break;
-                    next = (int)atomicAdd(a.counter, 1u);
-                    x.hk = item % a.kv_heads;
-                    const Seq s = find_sequence(a.cu, a.B, a.T, a.max_len, slots - 1 - item / a.kv_heads, two);
-                    x.start = s.start, x.len = s.len, x.tok0 = s.local * two;
-                    if (s.local < 0 || x.tok0 >= s.len) continue;
-                    x.kv_slot = s.start / KT + (s.first_slot - s.start / two);
-                    auto tiles = [&](int tok) {              // key tiles of the query tile that begins at this token
-                        return tok >= s.len ? 0 : ((a.causal ? min(s.len, tok + a.tokens) : s.len) + kWideKT - 1) / kWideKT;
-                    };
-                    x.nt_a = tiles(x.tok0), x.nt_b = tiles(x.tok0 + a.tokens);
-                    break;
-                }
-                const int ws = w & 1;
-                const uint32_t round = (uint32_t)(w >> 1) & 1u;
-                if (!mbar_wait_bounded(bar(W_WEMPTY + ws), round ^ 1u)) { ok = false; break; }
-                work[ws] = x;
-                mbar_arrive(bar(W_WFULL + ws));
-                if (x.nt_a < 0) break;
-                if (!mbar_wait_bounded(bar(W_QEMPTY + ws), round ^ 1u)) { ok = false; break; }
-                const int q_rows = a.tokens * a.group * D, q_at = base_s + Cfg::OFF_Q + ws * 2 * Cfg::Q_BYTES;
-                mbar_expect_tx(bar(W_QFULL + ws), x.nt_b > 0 ? 2 * q_rows : q_rows);
-                tma_load_3d(q_at, &tmQ, 0, x.hk * a.group, x.start + x.tok0, bar(W_QFULL + ws));
-                if (x.nt_b > 0) tma_load_3d(q_at + Cfg::Q_BYTES, &tmQ, 0, x.hk * a.group, x.start + x.tok0 + a.tokens, bar(W_QFULL + ws));
-                const int nt = max(x.nt_a, x.nt_b);
-                const long long sc0 = ((long long)x.hk * a.slots + x.kv_slot) * KT;
-                for (int j = 0; j < nt; ++j, ++t) {
-                    const int st = t % kRing, cs = t % kScaleRing;
-                    const uint32_t r = ((uint32_t)(t / kRing) & 1u) ^ 1u, cr = ((uint32_t)(t / kScaleRing) & 1u) ^ 1u;
-                    if (!mbar_wait_bounded(bar(W_KEMPTY + st), r) || !mbar_wait_bounded(bar(W_CEMPTY + cs), cr)) { ok = false; break; }
-                    mbar_expect_tx(bar(W_KFULL + st), Cfg::K_BYTES);
-                    tma_load_3d(base_s + Cfg::OFF_K + st * Cfg::K_BYTES, &tmK, 0, x.hk, x.start + j * kWideKT, bar(W_KFULL + st));
-                    mbar_expect_tx(bar(W_CFULL + cs), 2 * kWideKT * 4);
-                    const uint32_t c_at = base_s + Cfg::OFF_SCALES + cs * (2 * kWideKT * 4);
-                    bulk_g2s(c_at, a.sK + sc0 + j * kWideKT, kWideKT * 4, bar(W_CFULL + cs));
-                    bulk_g2s(c_at + kWideKT * 4, a.sV + sc0 + j * kWideKT, kWideKT * 4, bar(W_CFULL + cs));
-                    if (!mbar_wait_bounded(bar(W_VEMPTY + st), r)) { ok = false; break; }
-                    mbar_expect_tx(bar(W_VFULL + st), Cfg::V_BYTES);
+        // ================= work and loads: the warp finds the work, its first lane starts the copies =================
+        const int slots = a.T / two + a.B, items = slots * a.kv_heads;
+        int t = 0;                                           // key tiles loaded so far
+        int next = blockIdx.x;                               // the first of a CTA by its number, the others from the counter
+        WideWork x{};
+        // this pair to the other roles, then its queries, keys and values; false when a wait gave up
+        auto load = [&](int w) -> bool {
+            const int ws = w & 1;
+            const uint32_t round = (uint32_t)(w >> 1) & 1u;
+            if (!mbar_wait_bounded(bar(W_WEMPTY + ws), round ^ 1u)) return false;
+            work[ws] = x;
+            mbar_arrive(bar(W_WFULL + ws));
+            if (x.nt_a < 0) return true;
+            if (!mbar_wait_bounded(bar(W_QEMPTY + ws), round ^ 1u)) return false;
+            const int q_rows = a.tokens * a.group * D, q_at = base_s + Cfg::OFF_Q + ws * 2 * Cfg::Q_BYTES;
+            mbar_expect_tx(bar(W_QFULL + ws), x.nt_b > 0 ? 2 * q_rows : q_rows);
+            tma_load_3d(q_at, &tmQ, 0, x.hk * a.group, x.start + x.tok0, bar(W_QFULL + ws));
+            if (x.nt_b > 0) tma_load_3d(q_at + Cfg::Q_BYTES, &tmQ, 0, x.hk * a.group, x.start + x.tok0 + a.tokens, bar(W_QFULL + ws));
+            const int nt = max(x.nt_a, x.nt_b);
+            const long long sc0 = ((long long)x.hk * a.slots + x.kv_slot) * KT;
+            for (int j = 0; j < nt; ++j, ++t) {
+                const int st = t % kRing, cs = t % kScaleRing;
+                const uint32_t r = ((uint32_t)(t / kRing) & 1u) ^ 1u, cr = ((uint32_t)(t / kScaleRing) & 1u) ^ 1u;
+                if (!mbar_wait_bounded(bar(W_KEMPTY + st), r) || !mbar_wait_bounded(bar(W_CEMPTY + cs), cr)) return false;
+                mbar_expect_tx(bar(W_KFULL + st), Cfg::K_BYTES);
+                tma_load_3d(base_s + Cfg::OFF_K + st * Cfg::K_BYTES, &tmK, 0, x.hk, x.start + j * kWideKT, bar(W_KFULL + st));
+                mbar_expect_tx(bar(W_CFULL + cs), 2 * kWideKT * 4);
+                const uint32_t c_at = base_s + Cfg::OFF_SCALES + cs * (2 * kWideKT * 4);
+                bulk_g2s(c_at, a.sK + sc0 + j * kWideKT, kWideKT * 4, bar(W_CFULL + cs));
+                bulk_g2s(c_at + kWideKT * 4, a.sV + sc0 + j * kWideKT, kWideKT * 4, bar(W_CFULL + cs));
+                if (!mbar_wait_bounded(bar(W_VEMPTY + st), r)) return false;
+                mbar_expect_tx(bar(W_VFULL + st), Cfg::V_BYTES);
 #pragma unroll
-                    for (int sl = 0; sl < D / 64; ++sl)
-                        tma_load_2d(base_s + Cfg::OFF_V + st * Cfg::V_BYTES + sl * Cfg::V_SLAB, &tmV, sl * 128,
-                                    (int)(sc0 + j * kWideKT), bar(W_VFULL + st));
+                for (int sl = 0; sl < D / 64; ++sl)
+                    tma_load_2d(base_s + Cfg::OFF_V + st * Cfg::V_BYTES + sl * Cfg::V_SLAB, &tmV, sl * 128, (int)(sc0 + j * kWideKT),
+                                bar(W_VFULL + st));
+            }
+            return true;
+        };
+        for (int w = 0;; ++w) {
+            x.nt_a = -1;
+            while (next < items && x.nt_a < 0) {             // to a slot that has rows
+                const int item = next;
+                unsigned taken = 0u;
+                if (lane == 0) taken = atomicAdd(a.counter, 1u);
+                x.hk = item % a.kv_heads;
+                const Seq s = find_sequence(a.cu, a.B, a.T, a.max_len, slots - 1 - item / a.kv_heads, two);
+                next = (int)(gridDim.x + __shfl_sync(0xffffffffu, taken, 0));
+                x.start = s.start, x.len = s.len, x.tok0 = s.local * two;
+                if (s.local < 0 || x.tok0 >= s.len) continue;
+                x.kv_slot = s.start / KT + (s.first_slot - s.start / two);
+                auto tiles = [&](int tok) {                  // key tiles of the query tile that begins at this token
+                    return tok >= s.len ? 0 : ((a.causal ? min(s.len, tok + a.tokens) : s.len) + kWideKT - 1) / kWideKT;
+                };
+                x.nt_a = tiles(x.tok0), x.nt_b = tiles(x.tok0 + a.tokens);
+            }
+            int ok = 1;
+            if (lane == 0) {
+                ok = load(w) ? 1 : 0;
+                if (!ok) {                                   // copies in flight land before the block lets go of its memory
+                    note_timeout(a.status);
+                    for (int i = 0; i < kRing; ++i)
+                        for (uint32_t ph = 0; ph < 2; ++ph)
+                            mbar_wait_bounded(bar(W_KFULL + i), ph, 64u), mbar_wait_bounded(bar(W_VFULL + i), ph, 64u);
                 }
             }
-            if (!ok) {                                       // copies in flight land before the block lets go of its memory
-                note_timeout(a.status);
-                for (int i = 0; i < kRing; ++i)
-                    for (uint32_t ph = 0; ph < 2; ++ph)
-                        mbar_wait_bounded(bar(W_KFULL + i), ph, 64u), mbar_wait_bounded(bar(W_VFULL + i), ph, 64u);
-            }
+            if (!__shfl_sync(0xffffffffu, ok, 0) || x.nt_a < 0) break;
         }
     } else if (warp == 9) {
         // ================= MMA issuer =================
