@@ -32,6 +32,8 @@
 // so that every shared-memory address is a constant off three per-thread bases.
 // A row that one CTA scans whole is written there; a row cut between CTAs leaves at most two partial rows per CTA,
 // merged by a second kernel that is launched behind the first one's tail.
+// Measured: 32 requests up to 32768 positions, 32/8 heads, D 128, 64-position pages, 122-130 us a call (floor at the copy
+// rate: 95.8); 24 up to 4096, 12/12 heads, D 64: 19.7 us (6.8).  What bounds it is issue: 52 % of the slots, ALU pipe 54 %.
 #include "kv4.cuh"
 
 #include <cmath>
