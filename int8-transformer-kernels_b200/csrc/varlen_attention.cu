@@ -686,6 +686,10 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
         // ================= work and loads: the warp finds the work, its first lane starts the copies =================
+        // A choice with two sides, timed in turn against one lane that bisects: five prompts up to 67 tokens 9.8 against
+        // 10.2 us and four of 4096 at D 128 294.4 against 295.7, but 16 up to 2048 tokens 303.5 against 297.4 and eight of
+        // 4096 at D 64 481.5 against 478.8.  Keeping the counter's answer unused until the next pair is due did not bring
+        // those back (302.8 and 484.3).
         const int slots = a.T / two + a.B, items = slots * a.kv_heads;
         int t = 0;                                           // key tiles loaded so far
         int next = blockIdx.x;                               // the first of a CTA by its number, the others from the counter
