@@ -22,6 +22,7 @@
 //   keys' and values' scales as [key head][slot of 64] (coalesced for the softmax warps; in the caller's layout the
 //   scales of a head are a token apart).  A value scale that is not finite becomes a NaN key scale there: rows that
 //   see the position are NaN, rows that do not are untouched.
+#include "score_reference.cuh"
 #include "tcgen05.cuh"
 
 #include <cmath>
@@ -582,8 +583,9 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 // P.V in the order of the one thread that issues both.
 // The exponentials are taken against the reference of the tiles before, without looking for the maximum first; the
 // maximum is found on the way, and only where it runs more than kLazyStep ahead (the scores are still there) is the
-// reference moved, the accumulator rescaled and the tile done again.  The first reference of a row comes from its first
-// 32 scores.
+// reference moved, the accumulator rescaled and the tile done again, once: then no score is ahead by more than the
+// rounding of the reference.  Where that rounding would matter, far_tile() does the tile.  The first reference of a row
+// comes from its first 32 scores.
 // The pairs of tiles are taken from a counter, long rows first, by the thread that starts the loads, which runs ahead
 // into the next pair while the last one is finished.
 // (8192 tokens causal, 32/8 heads, D 128: 540 us, 1.02 PFLOP/s; with prefill_attention.cu's shape 622.  Two score blocks of
@@ -633,6 +635,66 @@ struct WideWork {
     int start, len, tok0, hk, kv_slot, nt_a, nt_b, pad;      // nt_a < 0: no more work
 };
 
+// A tile of which some row's scores are too far out for a reference of one fp32 number: its largest score first, then the
+// reference and what it changes, then the probabilities with the reference's remainder, four words of P over columns that
+// have been read.  In a function of its own, so that the common way keeps its registers; the steps and their order are
+// the same, so the other rows of the warp get the bits they get there.  Returns the row's reference and sum.  kFarMark
+// stands for a far reference, or for none yet, that is in *kept: against it any score that the row sees is ahead, so the
+// row's next tile comes here as well.
+constexpr float kFarMark = 3.402823466e38f;
+template <int D>
+__device__ __noinline__ float2 far_tile(uint32_t s_addr, uint32_t o_addr, const float* sk, int lim, float qscale, float lift, float nm, float l,
+                                        bool first, ScoreReference* kept) {
+    auto scores8 = [&](int c, float (&y)[8]) {
+        uint32_t sr[8];
+        tmem_ld8(s_addr + c, sr);
+        tmem_ld_wait(sr);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = c + e < lim ? (float)(int)sr[e] * sk[c + e] : -INFINITY;
+    };
+    float top = -INFINITY, y[8];
+#pragma unroll 1
+    for (int c = 0; c < kWideKT; c += 8) {
+        scores8(c, y);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, y[e]);
+    }
+    ScoreReference ref = nm == kFarMark ? *kept : ScoreReference{nm, 0.f, false};
+    float corr = 1.0f;
+    if (ref.exponent(top, qscale, lift) > lift + kLazyStep) corr = ex2_approx(ref.move_to(top, qscale, lift));
+    *kept = ref;
+    const bool mark = ref.far || ref.nm == INFINITY;
+    if (ref.nm == INFINITY) ref.nm = lift;           // no score yet: no probability either
+    if (!first) {
+        l *= corr;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 16) {
+            uint32_t o[16];
+            tmem_ld16(o_addr + c, o);
+            tmem_ld_wait(o);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * corr);
+            tmem_st16(o_addr + c, o);
+        }
+    }
+    const float* sv = sk + kWideKT;
+    f32x2 sum2 = pack2(0.f, 0.f);
+#pragma unroll 1
+    for (int c = 0; c < kWideKT; c += 8) {
+        scores8(c, y);
+        f32x2 p[4];
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            p[e] = pack2(ex2_approx(ref.exponent(y[2 * e], qscale, lift)), ex2_approx(ref.exponent(y[2 * e + 1], qscale, lift)));
+            w[e] = pack_h2(p[e].x * sv[c + 2 * e], p[e].y * sv[c + 2 * e + 1]);
+        }
+        sum2 = add2(sum2, add2(add2(p[0], p[1]), add2(p[2], p[3])));
+        tmem_st4(s_addr + c / 2, w[0], w[1], w[2], w[3]);
+    }
+    return make_float2(mark ? kFarMark : ref.nm, l + (sum2.x + sum2.y));
+}
+
 template <int D>
 __global__ void __launch_bounds__(kWideThreads, 1)
 varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
@@ -640,6 +702,7 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     using Cfg = WideCfg<D>;
     extern __shared__ unsigned char smem_raw[];
     __shared__ WideWork work[2];
+    __shared__ ScoreReference far_refs[256];                 // of a softmax thread
     const uint32_t raw_s = smem_u32(smem_raw);
     const uint32_t base_s = (raw_s + 1023u) & ~1023u;       // swizzle patterns are functions of address bits
     unsigned char* base = smem_raw + (base_s - raw_s);
@@ -872,7 +935,7 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             for (int o = 16; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
             const float lift = (float)min(100, max(-100, 6 - ((int)(__float_as_uint(most) >> 23) - 127)));
 
-            float nm = 0.f;                                  // lift less the reference (log2 units)
+            float nm = 0.f;                                  // the row's reference (ScoreReference), or kFarMark: it is in far_refs
             float l = 0.f;
             for (int j = 0; j < nt; ++j) {
                 const int cs = (t0 + j) % kScaleRing;
@@ -920,7 +983,7 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                             for (int e = 0; e < 4; ++e) m0 = max3(m0, y4[e].x, y4[e].y);
                         }
                         nm = lift - m0 * qscale;
-                        if (!(fabsf(nm) < 1e30f)) nm = lift; // (scores that are not finite: the row becomes NaN by itself)
+                        if (!(fabsf(nm) < kFarScore)) nm = kFarMark, far_refs[threadIdx.x] = ScoreReference{INFINITY, 0.f, false};
                     }
                     uint32_t P[64];
                     f32x2 sum2;
@@ -957,7 +1020,9 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
 #pragma unroll
                         for (int i = CHUNKS * 8; i < 64; ++i) P[i] = 0u;
                     };
-                    for (;;) {
+                    int turn = 0;
+#pragma unroll 1
+                    for (;; turn = 1) {
                         // a last tile that no row sees the second half of costs half (sixteen prompts up to 2048, 32/8 heads:
                         // 304 -> 295 us; at head_dim 64 the third form does not fit the registers: 482 -> 507 us for eight
                         // sequences of 4096, 8 heads)
@@ -965,11 +1030,17 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                         else if (D == 64 || tile_lim > 64) pass(std::true_type{}, std::integral_constant<int, 8>{});
                         else pass(std::true_type{}, std::integral_constant<int, 4>{});
                         const bool ahead = mx > lift + kLazyStep;
-                        if (!__any_sync(0xffffffffu, ahead)) break;
-                        // the reference moves to this tile's maximum, and the tile is done again; P.V of the tile before
+                        if (turn | !__any_sync(0xffffffffu, ahead)) break;
+                        // the reference moves to this tile's maximum, and the tile is done again, once; P.V of the tile before
                         // has retired (its commit came before that of these scores)
-                        const float up = ahead ? mx - lift : 0.f, corr = ex2_approx(-up);
-                        nm -= up;
+                        const float to = ahead ? nm - (mx - lift) : nm;
+                        if (__any_sync(0xffffffffu, nm == kFarMark || fabsf(to) >= kFarScore)) {
+                            const float2 r = far_tile<D>(s_addr, o_addr, sk, lim, qscale, lift, nm, l, j == 0, far_refs + threadIdx.x);
+                            nm = r.x, l = r.y;
+                            goto stored;
+                        }
+                        const float corr = ex2_approx(to - nm);
+                        nm = to;
                         l *= corr;
                         if (j > 0) {
                             uint32_t o[32];
@@ -986,6 +1057,7 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                     l += sum2.x + sum2.y;
                     tmem_st32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&P[0]));
                     tmem_st32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&P[32]));
+                stored:
                     tmem_st_wait();
                     tc_fence_before();
                 }
