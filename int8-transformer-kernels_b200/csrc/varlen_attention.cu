@@ -355,13 +355,14 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
         float* xch = reinterpret_cast<float*>(base + Cfg::OFF_XCH);                      // [2][half][row]
         float qscale = stored ? a.sQ[(long long)(s.start + tok) * a.sq_stride + head] * a.score_scale_log2 : 0.f;
         if (qscale == 0.f) qscale = 1e-30f;              // a removed position (-inf) stays removed under a scale of zero
-        const f32x2 qs2 = pack2(qscale, qscale);
         const int visible = a.causal ? min(s.len, tok + 1) : s.len;      // positions that this row sees
         const uint32_t lane_addr = tmem_base + ((uint32_t)(q * 32) << 16);
         constexpr uint32_t kMagicI = 0x4B400000u;        // 1.5 * 2^23: |q.k| < 2^22 converts by an add and a subtract
         const f32x2 nmagic2 = pack2(-12582912.f, -12582912.f);
         const long long sc0 = ((long long)hk * a.slots + kv_slot) * KT + half * HK + lane;
-        float m_ref = -INFINITY;
+        ScoreReference ref{INFINITY, 0.f, false};        // none yet: any score is ahead of it
+        float nm = 0.f;                                  // ref.nm once there is one
+        bool far_rows = false;                           // some row of the warp has a far reference
         f32x2 l2 = pack2(0.f, 0.f);
         bool ok = true;
 
@@ -409,8 +410,8 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 mx = fmaxf(mx, fmaxf(yy[e].x, yy[e].y));
             }
         };
-        // p = 2^(y*qscale - m_ref) for 8 columns; p * sV * c leaves as four fp16 pairs for this row's lane of the P tile
-        auto exp8 = [&](const f32x2* y4, const float* v8, f32x2 nm2, uint32_t dst) {
+        // p = 2^(y*qs + nm) for 8 columns; p * sV * c leaves as four fp16 pairs for this row's lane of the P tile
+        auto exp8 = [&](const f32x2* y4, const float* v8, f32x2 qs2, f32x2 nm2, uint32_t dst) {
             const float4 va = *reinterpret_cast<const float4*>(v8);
             const float4 vb = *reinterpret_cast<const float4*>(v8 + 4);
             const f32x2 x0 = fma2(y4[0], qs2, nm2), x1 = fma2(y4[1], qs2, nm2);
@@ -457,13 +458,19 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             // ---- row maximum across the two halves ----
             xch[(st * 2 + half) * kQT + r] = mx;
             asm volatile("bar.sync %0, 64;" ::"r"(1 + q) : "memory");
-            mx = fmaxf(mx, xch[(st * 2 + (half ^ 1)) * kQT + r]) * qscale;     // log2 units
+            mx = fmaxf(mx, xch[(st * 2 + (half ^ 1)) * kQT + r]);
 
-            const bool move = mx > m_ref + kLazyStep;
-            const float m_new = move ? mx : m_ref;
-            const float corr = move ? ex2_approx(m_ref - m_new) : 1.0f;
-            if (move) l2 = mul2(l2, pack2(corr, corr));
+            const bool move = fmaf(mx, qscale, ref.nm) + ref.rest > kLazyStep;
             const bool warp_moves = __any_sync(0xffffffffu, move);
+            float corr = 1.0f;
+            if (warp_moves) {
+                if (move) {
+                    corr = ex2_approx(ref.move_to(mx, qscale, 0.f));
+                    nm = ref.nm;
+                    l2 = mul2(l2, pack2(corr, corr));
+                }
+                far_rows = __any_sync(0xffffffffu, ref.far);
+            }
 
             // ---- this tile's P buffer is free once PV of tile j-2 retired; the accumulator is touched only when a
             // maximum moved, and then PV of tile j-1 must have retired too ----
@@ -487,11 +494,15 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 }
                 tmem_st_wait();
             }
-            m_ref = m_new;
-
             // ---- exponentials of this tile interleaved with the conversion of the NEXT tile's scores ----
             const uint32_t prow = lane_addr + Cfg::TM_P + st * (KT / 2) + half * (HK / 2);
-            const f32x2 nm2 = pack2(-m_ref, -m_ref);
+            f32x2 qs2 = pack2(qscale, qscale), nm2 = pack2(nm, nm);
+            if (far_rows) {          // the remainder of a far reference: the exponents are made here
+                const f32x2 rest2 = pack2(ref.rest, ref.rest);
+#pragma unroll
+                for (int e = 0; e < HK / 2; ++e) y[e] = add2(fma2(y[e], qs2, nm2), rest2);
+                qs2 = pack2(1.f, 1.f), nm2 = pack2(0.f, 0.f);
+            }
             const float* vsc = wsc + st * (2 * HK) + HK;
             mx = -INFINITY;
             if (has_next) {
@@ -512,7 +523,7 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 #pragma unroll
                     for (int h = 0; h < 2; ++h) {
                         const int c = cc * 2 + h;
-                        exp8(&y[c * 4], vsc + c * 8, nm2, prow + c * 4);
+                        exp8(&y[c * 4], vsc + c * 8, qs2, nm2, prow + c * 4);
                         convert8(&sr[cc & 1][h * 8], ksc + c * 8, &y[c * 4], mx);
                     }
                 }
@@ -522,7 +533,7 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                 if (lane == 0) mbar_arrive(bar(B_SEMPTY + sb1));
             } else {
 #pragma unroll
-                for (int c = 0; c < HK / 8; ++c) exp8(&y[c * 4], vsc + c * 8, nm2, prow + c * 4);
+                for (int c = 0; c < HK / 8; ++c) exp8(&y[c * 4], vsc + c * 8, qs2, nm2, prow + c * 4);
             }
             tmem_st_wait();
             tc_fence_before();

@@ -54,7 +54,7 @@ def _check_varlen(out, args, lens, causal):
     return single
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 @pytest.mark.parametrize("e", [16, 21, 23, 26, 28, 31, 40, 64, 100])
 def test_varlen_large_scores(D, e):
     op, lens = ext().int8_attention_varlen, [300, 7, 129]
@@ -68,7 +68,7 @@ def test_varlen_large_scores(D, e):
     ext().check_status()
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_varlen_scores_become_large_on_the_way(D):
     """Some keys, some queries, or the keys of a later tile only: rows with and without large scores side by side."""
     op, lens = ext().int8_attention_varlen, [420]
@@ -87,7 +87,7 @@ def test_varlen_scores_become_large_on_the_way(D):
     ext().check_status()
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_varlen_equal_largest_scores_share_the_row(D):
     args = _codes(200, 2, 1, D, seed=3)
     args[1][[20, 90, 150]] = args[0][40:41, :1]                                # the key that fits query 40 best, three times
@@ -102,7 +102,7 @@ def test_varlen_equal_largest_scores_share_the_row(D):
     assert torch.isfinite(out).all()
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_varlen_an_infinite_score_is_nan_in_its_rows_only(D):
     base = _codes(300, 2, 1, D, seed=4)
     good = ext().int8_attention_varlen(*base, _cu([300]), 300, True)
@@ -113,7 +113,7 @@ def test_varlen_an_infinite_score_is_nan_in_its_rows_only(D):
     assert out[200].isnan().all() and torch.equal(out[keep], good[keep])
 
 
-@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("D", [64, 128, 256])
 def test_varlen_scores_of_minus_infinity_are_left_out(D):
     """Key scales of infinity where the products are negative: no probability, in the first tile or later, and a row that
     has only such scores at first starts where it has others."""
