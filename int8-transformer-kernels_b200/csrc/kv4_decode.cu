@@ -35,6 +35,7 @@
 // Measured: 32 requests up to 32768 positions, 32/8 heads, D 128, 64-position pages, 122-130 us a call (floor at the copy
 // rate: 95.8); 24 up to 4096, 12/12 heads, D 64: 19.7 us (6.8).  What bounds it is issue: 52 % of the slots, ALU pipe 54 %.
 #include "kv4.cuh"
+#include "score_reference.cuh"
 
 #include <cmath>
 
@@ -50,7 +51,7 @@ constexpr int kScanThreads = kWarps * 32;
 // below its largest score times the largest scale met so far, and moves when a product would run kSlack above that.
 constexpr float kTop = 13.0f, kSlack = 2.0f;
 constexpr int kLeastScale = -20;          // log2 of the scale assumed for values that have none (p itself stays below 2^35)
-constexpr float kNoReference = 1e30f;       // negative reference of a row that has met nothing: 2^(-inf + 1e30) is still 0
+constexpr float kNoReference = 3e38f;       // negative reference of a row that has met nothing: 2^(-inf + 3e38) is still 0
 
 template <int D, int NT, int W>             // NT: blocks of 8 query heads per key head; W: copies of the heads in a block
 struct Kv4Cfg {
@@ -493,8 +494,9 @@ kv4_scan_kernel(const Kv4Args a) {
                         mx.x = fmaxf(mx.x, __shfl_xor_sync(0xffffffffu, mx.x, o));
                         mx.y = fmaxf(mx.y, __shfl_xor_sync(0xffffffffu, mx.y, o));
                     }
-                    // the reference goes up to kTop - (largest scale) below the largest score, never down
-                    const f32x2 to = pack2(fminf(neg[n].x, room - kSlack - mx.x), fminf(neg[n].y, room - kSlack - mx.y));
+                    // the reference goes up to kTop - (largest scale) below the largest score (to the score itself where
+                    // that offset would be rounded away: p * s is then at most s), never down
+                    const f32x2 to = pack2(fminf(neg[n].x, negative_reference(mx.x, room - kSlack)), fminf(neg[n].y, negative_reference(mx.y, room - kSlack)));
                     const f32x2 keep = pack2(ex2_approx(to.x - neg[n].x), ex2_approx(to.y - neg[n].y));
                     neg[n] = to;
                     l2[n] = mul2(l2[n], keep);

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from helpers import ext
+from oracle import grouped as og
 
 pytestmark = pytest.mark.gpu
 
@@ -129,3 +130,59 @@ def test_varlen_scores_of_minus_infinity_are_left_out(D):
     want, spread = p @ vv, p @ np.abs(vv)
     slack = 1.05 * (2.0 ** -11 * (spread + np.abs(want)) + 51 * 2.0 ** -31 * np.abs(v[:251, 0] * sv[:251, 0, None]).max() + 2.0 ** -25)
     assert (np.abs(out[250, 0].double().cpu().numpy() - want) <= slack).all()
+
+
+# ---- 4-bit decode ------------------------------------------------------------------------------------
+def _cache(lens, kv, D, page, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    need = [-(-n // page) for n in lens]
+    pool = torch.zeros(sum(need), kv, ext().int4_kv_block_bytes(page, D), dtype=torch.uint8, device="cuda")
+    order = torch.randperm(sum(need), device="cuda", generator=g).int()
+    table, at = torch.zeros(len(lens), max(need), dtype=torch.int32, device="cuda"), 0
+    for b, n in enumerate(lens):
+        table[b, :need[b]] = order[at:at + need[b]]
+        pos = torch.arange(n, device="cuda")
+        slots = table[b, (pos // page)].long() * page + pos % page
+        k, v = (torch.randn(n, kv, D, device="cuda", generator=g).half() for _ in range(2))
+        ext().kv_append_quantize_int4(k, v, pool, slots, page)
+        at += need[b]
+    return pool, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
+
+
+def _rows(pool, table, b, h, n, page, D):
+    blocks = [og.int4_unblock(pool[p, h], page, D) for p in table[b, :-(-n // page)]]
+    return [[np.concatenate([blk[i][x] for blk in blocks])[:n].astype(np.float64) for x in range(3)] for i in (0, 1)]
+
+
+@pytest.mark.parametrize("H,kv,D,page,lens", [(4, 4, 64, 16, [3000, 1]), (8, 2, 128, 32, [300, 5, 129]), (4, 2, 128, 128, [2, 700]), (24, 2, 64, 64, [400]),
+                                              (7, 1, 64, 16, [129, 64])])
+@pytest.mark.parametrize("e", [16, 21, 23, 26, 28, 31, 40, 64, 100])
+def test_int4_decode_large_scores(H, kv, D, page, lens, e):
+    """A score is put together from s (q . c - 8 Q) + z Q per group, with up to eight roundings of half a step (2^-24) of
+    these parts.  p * s is rounded to fp16 (2^-11 of up to 8 steps s), the result too; where p * s is below the range,
+    half the smallest fp16 number (2^-25) times 8 for each candidate."""
+    pool, table, ln = _cache(lens, kv, D, page, seed=H + D)
+    q, sq = ext().quantize_per_token(torch.randn(len(lens), H, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(e)))
+    far = sq * 2.0 ** e
+    if e % 2 == 0:
+        far[:, ::2] = sq[:, ::2]                                               # every other head as it was
+    out = ext().int4_decode_attention_paged(q, far, pool, table, ln, max(lens), page)
+    got, qn, sn, pn, tn = out.double().cpu().numpy(), q.double().cpu().numpy(), far.double().cpu().numpy(), pool.cpu().numpy(), table.cpu().numpy()
+    assert np.isfinite(got).all()
+    single = 0
+    for b, n in enumerate(lens):
+        for j in range(H):
+            (kc, ks, kz), (vc, vs, vz) = _rows(pn, tn, b, j // (H // kv), n, page, D)
+            qg = qn[b, j].reshape(-1, 64)
+            dot, total = np.einsum("lgc,gc->lg", kc.reshape(n, -1, 64), qg), qg.sum(-1)
+            unit = sn[b, j] * np.log2(np.e) / np.sqrt(D)
+            s = unit * (ks * (dot - 8 * total) + kz * total).sum(-1)
+            size = unit * (ks * (np.abs(dot) + 8 * np.abs(total)) + np.abs(kz * total)).sum(-1).max()
+            v = og.int4_values(vc, vs, vz)
+            near = s >= s.max() - 2 * 8 * 2.0 ** -24 * size - 50
+            slack = 1.05 * (2.0 ** -11 * (8 * vs[near].max() + np.abs(v[near]).max()) + 2.0 ** -22 * near.sum() + 2.0 ** -50 * n * np.abs(v).max())
+            assert (v[near].min(0) - slack <= got[b, j]).all() and (got[b, j] <= v[near].max(0) + slack).all(), (b, j)
+            single += near.sum() == 1
+    assert single > 0.3 * len(lens) * H
+    assert torch.equal(out, ext().int4_decode_attention_paged(q, far, pool, table, ln, max(lens), page))
+    ext().check_status()
