@@ -133,7 +133,7 @@ def test_varlen_scores_of_minus_infinity_are_left_out(D):
 
 
 # ---- 4-bit decode ------------------------------------------------------------------------------------
-def _cache(lens, kv, D, page, seed):
+def _cache(lens, kv, D, page, seed, f=1.0):
     g = torch.Generator(device="cuda").manual_seed(seed)
     need = [-(-n // page) for n in lens]
     pool = torch.zeros(sum(need), kv, ext().int4_kv_block_bytes(page, D), dtype=torch.uint8, device="cuda")
@@ -143,7 +143,8 @@ def _cache(lens, kv, D, page, seed):
         table[b, :need[b]] = order[at:at + need[b]]
         pos = torch.arange(n, device="cuda")
         slots = table[b, (pos // page)].long() * page + pos % page
-        k, v = (torch.randn(n, kv, D, device="cuda", generator=g).half() for _ in range(2))
+        k, v = (torch.randn(n, kv, D, device="cuda", generator=g) for _ in range(2))
+        k, v = k.half(), (v * f).half()
         ext().kv_append_quantize_int4(k, v, pool, slots, page)
         at += need[b]
     return pool, table, torch.tensor(lens, dtype=torch.int32, device="cuda")
@@ -156,12 +157,13 @@ def _rows(pool, table, b, h, n, page, D):
 
 @pytest.mark.parametrize("H,kv,D,page,lens", [(4, 4, 64, 16, [3000, 1]), (8, 2, 128, 32, [300, 5, 129]), (4, 2, 128, 128, [2, 700]), (24, 2, 64, 64, [400]),
                                               (7, 1, 64, 16, [129, 64])])
-@pytest.mark.parametrize("e", [16, 21, 23, 26, 28, 31, 40, 64, 100])
-def test_int4_decode_large_scores(H, kv, D, page, lens, e):
+@pytest.mark.parametrize("e,f", [(16, 1.0), (21, 2.0 ** -9), (23, 1.0), (24, 16.0), (25, 4.0), (26, 2.0 ** -5), (27, 2.0 ** -7), (28, 2.0 ** -9), (31, 1.0),
+                                 (40, 64.0), (64, 1.0), (100, 1.0)])
+def test_int4_decode_large_scores(H, kv, D, page, lens, e, f):
     """A score is put together from s (q . c - 8 Q) + z Q per group, with up to eight roundings of half a step (2^-24) of
     these parts.  p * s is rounded to fp16 (2^-11 of up to 8 steps s), the result too; where p * s is below the range,
-    half the smallest fp16 number (2^-25) times 8 for each candidate."""
-    pool, table, ln = _cache(lens, kv, D, page, seed=H + D)
+    half the smallest fp16 number (2^-25) times 8 for each candidate.  The values' size moves the reference."""
+    pool, table, ln = _cache(lens, kv, D, page, H + D, f)
     q, sq = ext().quantize_per_token(torch.randn(len(lens), H, D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(e)))
     far = sq * 2.0 ** e
     if e % 2 == 0:
