@@ -423,7 +423,9 @@ enum i8tk_dtype { I8TK_F16 = 0, I8TK_BF16 = 1 };
  *              [0, rope_rows) turns the rotated rows of its token into NaN (scales, when quantised).
  *   out        [tokens, heads + kv_heads, head_dim], qkv's type (value heads are not copied)
  *   codes      int8 [tokens, heads + 2*kv_heads, head_dim], scales fp32 [tokens, heads + 2*kv_heads]:
- *              max(absmax, 1e-8)/127 and rne(y/scale), as i8tk_quantize_per_token_f32 gives for y
+ *              max(absmax, 1e-8)/127 and rne(y/scale), as i8tk_quantize_per_token_f32 gives for y.  A query or
+ *              key head with a NaN or an infinity that is normed or rotated gets a NaN scale; the others
+ *              follow that quantiser's rule for such values.
  *   k_out      [tokens, kv_heads, head_dim] of qkv's type or NULL: the keys unquantised as well (for
  *              i8tk_kv4_append)
  * head_dim 64, 128 or 256; rotary_dim a multiple of 16, at most head_dim; row_stride a multiple of

@@ -74,6 +74,18 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
+// maximum that is NaN when an operand is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // ROT: 0 no rotation, 1 half-split pairs, 2 interleaved pairs.
 template <typename T, int D, bool QUANT, int ROT>
 __global__ void __launch_bounds__(kThreads, 8)
@@ -117,13 +129,6 @@ qk_norm_rope_kernel(const QkArgs a) {
             if (sub == 0) scales[i * GROUPS] = scale;
         }
     };
-    auto row_max = [&](const f32x2* u) {
-        float mx = max3(max3(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y),
-                        max3(fabsf(u[2].x), fabsf(u[2].y), fmaxf(fabsf(u[3].x), fabsf(u[3].y))));
-#pragma unroll
-        for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        return mx;
-    };
 
     if (QUANT && (kind == 2 || (ROT == 0 && a.q_weight == nullptr))) {
         // rows that are only quantised get exactly the per-token quantiser: a quotient next to a tie is divided
@@ -131,7 +136,12 @@ qk_norm_rope_kernel(const QkArgs a) {
         for (int i = 0; i < kRows; ++i) {
             if (unit0 + i * GROUPS >= count) break;  // the whole warp is past the last head
             const f32x2 u[4] = {widen(tag, raw[i].x), widen(tag, raw[i].y), widen(tag, raw[i].z), widen(tag, raw[i].w)};
-            const float scale = div127(fmaxf(row_max(u), 1e-8f)), inv = rcp_approx(scale);
+            float mx = max3(max3(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y),
+                            max3(fabsf(u[2].x), fabsf(u[2].y), fmaxf(fabsf(u[3].x), fabsf(u[3].y))));
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            mx = fmaxf(mx, 1e-8f);
+            const float scale = mx < INFINITY ? div127(mx) : mx, inv = rcp_approx(scale);
             const f32x2 inv2 = pack2(inv, inv);
             f32x2 q[4];
             float off = 0.f;
@@ -240,7 +250,13 @@ qk_norm_rope_kernel(const QkArgs a) {
                 *reinterpret_cast<uint4*>(out + i * GROUPS * D) =
                     make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
         } else {
-            const float scale = known ? div127(fmaxf(row_max(u) * r, 1e-8f)) : __int_as_float(0x7fc00000);
+            // a NaN or an infinity anywhere in the head makes the scale NaN (the product with r = 0 of an infinity is NaN, and
+            // so is div127 of one)
+            float mx = max3_nan(max3_nan(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y),
+                                max3_nan(fabsf(u[2].x), fabsf(u[2].y), max_nan(fabsf(u[3].x), fabsf(u[3].y))));
+#pragma unroll
+            for (int o = LPR / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float scale = known ? div127(max_nan(mx * r, 1e-8f)) : __int_as_float(0x7fc00000);
             const float inv = rcp_approx(scale) * r;
             const f32x2 inv2 = pack2(inv, inv);
             f32x2 q[4];
