@@ -729,9 +729,7 @@ struct Kv4Layout {
     size_t prefix_off, noted_off, parts_off, total;
 };
 
-int resident_ctas(int group) {
-    return group <= 2 ? Kv4Cfg<128, 1, 4>::CTAS : group <= 4 ? Kv4Cfg<128, 1, 2>::CTAS : group <= 8 ? Kv4Cfg<128, 1, 1>::CTAS : Kv4Cfg<128, 2, 1>::CTAS;
-}
+int resident_ctas(int group) { return group <= 8 ? Kv4Cfg<128, 1, 1>::CTAS : Kv4Cfg<128, 2, 1>::CTAS; }
 
 Kv4Layout kv4_layout(int B, int kv_heads, int group, int max_len, int D) {
     Kv4Layout y;

@@ -39,12 +39,12 @@ constexpr int kThreads = (2 + kSoftmaxWarps) * 32;
 constexpr int kRing = 3;
 constexpr float kLazyStep = 8.0f;        // log2 units the true maximum may run ahead of the reference: p <= 2^8, P < 2^15
 
-template <int D>
+// head_dim 256 (64 and 128: WideCfg)
 struct VarCfg {
-    static constexpr int ROW_BYTES = D < 128 ? D : 128;
-    static constexpr int QK_SLABS = D / ROW_BYTES;
-    static constexpr int Q_SLAB = kQT * ROW_BYTES;
-    static constexpr int K_SLAB = KT * ROW_BYTES;
+    static constexpr int D = 256;
+    static constexpr int QK_SLABS = D / 128;
+    static constexpr int Q_SLAB = kQT * 128;
+    static constexpr int K_SLAB = KT * 128;
     static constexpr int Q_BYTES = kQT * D;
     static constexpr int K_BYTES = KT * D;
     static constexpr int V_BYTES = KT * D * 2;
@@ -57,13 +57,11 @@ struct VarCfg {
     static constexpr int OFF_BARS = OFF_XCH + 2 * 2 * kQT * 4;
     static constexpr int NUM_BARS = 24;
     static constexpr int SMEM_BYTES = 1024 + OFF_BARS + NUM_BARS * 8 + 16;
-    static constexpr int CTAS_PER_SM = D == 256 ? 1 : 2;
-    static constexpr int NSB = D == 128 ? 1 : 2;            // score tiles: the second one would cost D = 128 its second CTA
-    static constexpr int TM_P = NSB * KT;
-    static constexpr int TM_O = D == 256 ? 256 : TM_P + KT;
-    static constexpr int TMEM_COLS = TM_O + D <= 256 ? 256 : 512;
-    static_assert(TM_P + KT <= TM_O && TM_O + D <= TMEM_COLS && TMEM_COLS * CTAS_PER_SM <= 512, "tensor-memory layout");
-    static_assert(SMEM_BYTES * CTAS_PER_SM <= 227 * 1024, "shared memory of an SM");
+    static constexpr int TM_P = 2 * KT;                                        // behind two score tiles
+    static constexpr int TM_O = 256;
+    static constexpr int TMEM_COLS = 512;
+    static_assert(TM_P + KT <= TM_O && TM_O + D <= TMEM_COLS, "tensor-memory layout");
+    static_assert(SMEM_BYTES <= 227 * 1024, "shared memory of an SM");
 };
 
 enum Bar : int {
@@ -211,11 +209,11 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-template <int D>
-__global__ void __launch_bounds__(kThreads, VarCfg<D>::CTAS_PER_SM)
+__global__ void __launch_bounds__(kThreads, 1)
 varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                         const __grid_constant__ CUtensorMap tmV, const __grid_constant__ Packed a) {
-    using Cfg = VarCfg<D>;
+    using Cfg = VarCfg;
+    constexpr int D = Cfg::D;
     extern __shared__ unsigned char smem_raw[];
     const uint32_t raw_s = smem_u32(smem_raw);
     const uint32_t base_s = (raw_s + 1023u) & ~1023u;       // swizzle patterns are functions of address bits
@@ -319,9 +317,9 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             // Q.K^T runs two tiles ahead of P.V (the softmax warps convert tile j + 1 while they exponentiate tile j)
             for (int j = 0; j < nt + 2 && ok; ++j) {
                 if (j < nt) {
-                    const int st = j % Cfg::NSB, kst = j % kRing;
+                    const int st = j & 1, kst = j % kRing;
                     if (!mbar_wait_spin_bounded(bar(B_KFULL + kst), (j / kRing) & 1) ||
-                        !mbar_wait_spin_bounded(bar(B_SEMPTY + st), ((j / Cfg::NSB) & 1) ^ 1)) {
+                        !mbar_wait_spin_bounded(bar(B_SEMPTY + st), ((j >> 1) & 1) ^ 1)) {
                         ok = false;
                         break;
                     }
@@ -331,9 +329,7 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
                     for (int k = 0; k < D / 32; ++k) {
                         const uint32_t qa = base_s + Cfg::OFF_Q + (k / 4) * Cfg::Q_SLAB;
                         const uint32_t ka = ks + (k / 4) * Cfg::K_SLAB;
-                        const uint64_t da = (D >= 128) ? smem_desc_sw128(qa) : smem_desc_sw64(qa);
-                        const uint64_t db = (D >= 128) ? smem_desc_sw128(ka) : smem_desc_sw64(ka);
-                        mma_i8(tmem_base + st * KT, da + 2 * (k % 4), db + 2 * (k % 4), idesc_qk, k != 0);
+                        mma_i8(tmem_base + st * KT, smem_desc_sw128(qa) + 2 * (k % 4), smem_desc_sw128(ka) + 2 * (k % 4), idesc_qk, k != 0);
                     }
                     tc_commit(bar(B_KEMPTY + kst));
                     tc_commit(bar(B_SFULL + st));
@@ -508,8 +504,8 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
             if (has_next) {
                 commit_scales(j + 1);
                 if (j + 2 < nt) prefetch(j + 2);
-                const int sb1 = (j + 1) % Cfg::NSB;
-                const bool got = mbar_wait_spin_bounded(bar(B_SFULL + sb1), ((j + 1) / Cfg::NSB) & 1);
+                const int sb1 = st ^ 1;
+                const bool got = mbar_wait_spin_bounded(bar(B_SFULL + sb1), ((j + 1) >> 1) & 1);
                 if (!__all_sync(0xffffffffu, got)) { ok = false; break; }
                 tc_fence_after();
                 const float* ksc = wsc + (st ^ 1) * (2 * HK);
@@ -1173,7 +1169,7 @@ int launch_varlen(const int8_t* Q, long long q_stride, const int8_t* K, long lon
         if constexpr (kWide)
             I8TK_CUDA(cudaFuncSetAttribute(varlen_wide_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, WideCfg<D>::SMEM_BYTES));
         else
-            I8TK_CUDA(cudaFuncSetAttribute(varlen_attention_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, VarCfg<D>::SMEM_BYTES));
+            I8TK_CUDA(cudaFuncSetAttribute(varlen_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, VarCfg::SMEM_BYTES));
         sms[dev] = n;
     }
     const VarLayout y = var_layout(a.T, a.B, a.kv_heads, D);
@@ -1201,7 +1197,7 @@ int launch_varlen(const int8_t* Q, long long q_stride, const int8_t* K, long lon
                                WideCfg<D>::SMEM_BYTES, st, tmQ, tmK, tmV, a));
     } else {
         const unsigned ctas = (unsigned)((a.T / a.tokens + a.B) * (long long)a.kv_heads);
-        I8TK_CUDA(launch_after(varlen_attention_kernel<D>, dim3(ctas), dim3(kThreads), VarCfg<D>::SMEM_BYTES, st, tmQ, tmK, tmV, a));
+        I8TK_CUDA(launch_after(varlen_attention_kernel, dim3(ctas), dim3(kThreads), VarCfg::SMEM_BYTES, st, tmQ, tmK, tmV, a));
     }
     return I8TK_OK;
 }
