@@ -11,18 +11,13 @@
 // exactly one word of the row.  A thread takes the key row and the value row of a token together.
 // Measured: 16384 tokens, 8 heads, D 128 (86 MB): append 29-30 us, read-back 16-18 us, both at 74 % of the issue slots.
 #include "kv4.cuh"
-
-#include <cuda_bf16.h>
+#include "pairs16.cuh"
 
 namespace i8tk {
 namespace {
 
 constexpr int kThreads = 128;
 
-__device__ __forceinline__ float2 widen(const __half*, uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ float2 widen(const __nv_bfloat16*, uint32_t v) {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
 // minimum of the pairs in two words; the sign bits of a word flipped
 __device__ __forceinline__ uint32_t min2(const __half*, uint32_t a, uint32_t b) {
     const __half2 m = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
@@ -31,17 +26,6 @@ __device__ __forceinline__ uint32_t min2(const __half*, uint32_t a, uint32_t b) 
 __device__ __forceinline__ uint32_t min2(const __nv_bfloat16*, uint32_t a, uint32_t b) {
     const __nv_bfloat162 m = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&m);
-}
-// x / 15 correctly rounded: a quotient from the rounded reciprocal, corrected by its exact remainder (Markstein)
-__device__ __forceinline__ float div15(float x) {
-    const float r = 1.0f / 15.0f;
-    const float q = x * r;
-    return fmaf(fmaf(-15.0f, q, x), r, q);
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // Codes and pair of the eight channels of this lane in its group of eight lanes.
@@ -57,7 +41,7 @@ __device__ __forceinline__ uint32_t quantize8(uint4 raw, __half2& pair) {
     for (int o = 4; o > 0; o >>= 1) both = min2(tag, both, __shfl_xor_sync(0xffffffffu, both, o));
     // the pair is fp16: a range that does not fit saturates
     const float lo = fminf(fmaxf(widen(tag, both).x, -65504.f), 65504.f), hi = fminf(fmaxf(-widen(tag, both).y, -65504.f), 65504.f);
-    const __half sh = __float2half_rn(div15(__fsub_rn(hi, lo)));
+    const __half sh = __float2half_rn(div_by<15>(__fsub_rn(hi, lo)));
     const float s = __half2float(sh);
     const __half zh = __float2half_rn(__fadd_rn(lo, 8.0f * s));
     const float z = __half2float(zh);

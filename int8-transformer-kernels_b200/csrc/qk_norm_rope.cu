@@ -19,9 +19,7 @@
 // A row is held by D/8 lanes, eight channels (one 16-byte load) each; a warp has kRows rows per lane group in flight.
 // Measured: 8192 bf16 tokens, 32/8 heads, D 128, quantised: 44-45 us for 156 MB, 71 % of the issue slots (84 us before the
 // norm, weight and rotation were joined and the kinds of rotation split).
-#include "common.cuh"
-
-#include <cuda_bf16.h>
+#include "pairs16.cuh"
 
 namespace i8tk {
 namespace {
@@ -49,10 +47,6 @@ struct QkArgs {
     void* k_out;                  // [tokens][kv_heads][D] in the input's type, or null (quantised form)
 };
 
-__device__ __forceinline__ float2 widen(const __half*, uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
-__device__ __forceinline__ float2 widen(const __nv_bfloat16*, uint32_t v) {
-    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-}
 __device__ __forceinline__ uint32_t narrow(const __half*, float a, float b) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -60,18 +54,6 @@ __device__ __forceinline__ uint32_t narrow(const __half*, float a, float b) {
 __device__ __forceinline__ uint32_t narrow(const __nv_bfloat16*, float a, float b) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
-}
-
-// x / 127 correctly rounded: a quotient from the rounded reciprocal, corrected by its exact remainder (Markstein)
-__device__ __forceinline__ float div127(float x) {
-    const float r = 1.0f / 127.0f;
-    const float q = x * r;
-    return fmaf(fmaf(-127.0f, q, x), r, q);
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
 }
 
 // maximum that is NaN when an operand is
@@ -141,7 +123,7 @@ qk_norm_rope_kernel(const QkArgs a) {
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
             mx = fmaxf(mx, 1e-8f);
-            const float scale = mx < INFINITY ? div127(mx) : mx, inv = rcp_approx(scale);
+            const float scale = mx < INFINITY ? div_by<127>(mx) : mx, inv = rcp_approx(scale);
             const f32x2 inv2 = pack2(inv, inv);
             f32x2 q[4];
             float off = 0.f;
@@ -251,12 +233,12 @@ qk_norm_rope_kernel(const QkArgs a) {
                     make_uint4(narrow(tag, u[0].x, u[0].y), narrow(tag, u[1].x, u[1].y), narrow(tag, u[2].x, u[2].y), narrow(tag, u[3].x, u[3].y));
         } else {
             // a NaN or an infinity anywhere in the head makes the scale NaN (the product with r = 0 of an infinity is NaN, and
-            // so is div127 of one)
+            // so is div_by of one)
             float mx = max3_nan(max3_nan(fabsf(u[0].x), fabsf(u[0].y), fabsf(u[1].x)), fabsf(u[1].y),
                                 max3_nan(fabsf(u[2].x), fabsf(u[2].y), max_nan(fabsf(u[3].x), fabsf(u[3].y))));
 #pragma unroll
             for (int o = LPR / 2; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float scale = known ? div127(max_nan(mx * r, 1e-8f)) : __int_as_float(0x7fc00000);
+            const float scale = known ? div_by<127>(max_nan(mx * r, 1e-8f)) : __int_as_float(0x7fc00000);
             const float inv = rcp_approx(scale) * r;
             const f32x2 inv2 = pack2(inv, inv);
             f32x2 q[4];
