@@ -101,6 +101,35 @@ struct Seq {
     int whole;                   // length before it is cut to max_len
 };
 __device__ __forceinline__ int cu_at(const int* cu, int i, int T) { return min(max(__ldg(cu + i), 0), T); }
+__device__ __forceinline__ Seq sequence_of(int from, int to, int found, int max_len, int slot, int n) {
+    Seq s;
+    s.start = from;
+    s.whole = max(to - from, 0);
+    s.len = min(s.whole, max_len);
+    s.first_slot = from / n + found;
+    s.local = slot - s.first_slot;
+    return s;
+}
+// One lane looks: seven probes a round, whose loads are on their way together.
+__device__ __forceinline__ Seq find_sequence_alone(const int* cu, int B, int T, int max_len, int slot, int n) {
+    int lo = 0, hi = B - 1;                  // largest b with cu[b] / n + b <= slot, or 0
+    while (lo < hi) {
+        const int step = (hi - lo + 8) >> 3;
+        int from[7], run = 0;
+#pragma unroll
+        for (int k = 0; k < 7; ++k) from[k] = cu_at(cu, min(lo + (k + 1) * step, hi), T);
+        bool below = true;
+#pragma unroll
+        for (int k = 0; k < 7; ++k) {        // the unbroken run of probes at or below the slot (a damaged table may break it)
+            const int b = min(lo + (k + 1) * step, hi);
+            below = below && from[k] < (long long)(slot - b + 1) * n;
+            run += below ? 1 : 0;
+        }
+        lo = min(lo + run * step, hi);
+        hi = run == 7 ? hi : min(lo + step - 1, hi);
+    }
+    return sequence_of(cu_at(cu, lo, T), cu_at(cu, lo + 1, T), lo, max_len, slot, n);
+}
 // A whole warp looks: 32 probes a round, so up to 32 sequences cost one load's latency, up to 1024 two.
 __device__ __forceinline__ Seq find_sequence(const int* cu, int B, int T, int max_len, int slot, int n) {
     const int lane = threadIdx.x & 31;
@@ -112,14 +141,7 @@ __device__ __forceinline__ Seq find_sequence(const int* cu, int B, int T, int ma
         // the last probe of the unbroken run from lane 0 on (a damaged table may break it)
         const int run = below == 0xffffffffu ? 32 : __ffs((int)~below) - 1, at = max(run - 1, 0);
         if (step == 1) {
-            Seq s;
-            const int found = min(lo + at, hi);
-            s.start = __shfl_sync(0xffffffffu, from, at);
-            s.whole = max(__shfl_sync(0xffffffffu, to, at) - s.start, 0);
-            s.len = min(s.whole, max_len);
-            s.first_slot = s.start / n + found;
-            s.local = slot - s.first_slot;
-            return s;
+            return sequence_of(__shfl_sync(0xffffffffu, from, at), __shfl_sync(0xffffffffu, to, at), min(lo + at, hi), max_len, slot, n);
         }
         lo = min(lo + at * step, hi);
         hi = min(lo + step - 1, hi);
@@ -755,11 +777,11 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
     if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
     if (warp == 8) {
-        // ================= work and loads: the warp finds the work, its first lane starts the copies =================
-        // A choice with two sides, timed in turn against one lane that bisects: five prompts up to 67 tokens 9.8 against
-        // 10.2 us and four of 4096 at D 128 294.4 against 295.7, but 16 up to 2048 tokens 303.5 against 297.4 and eight of
-        // 4096 at D 64 481.5 against 478.8.  Keeping the counter's answer unused until the next pair is due did not bring
-        // those back (302.8 and 484.3).
+        // ================= work and loads, by one lane =================
+        // A choice with two sides, timed in turn.  With the whole warp searching (find_sequence) 16 prompts up to 2048 tokens
+        // take 309 us instead of 299.5, 64 up to 1000 425 instead of 410, eight of 4096 at D 64 352 instead of 338, one of
+        // 8192 at D 128 538 instead of 530; 700 up to 60 tokens, 16/4 heads, 117 instead of 123.  One lane that bisects:
+        // 296, 404, 336, 530 and 134; fifteen probes a round: 305, 423, 342, 543 and 149.
         const int slots = a.T / two + a.B, items = slots * a.kv_heads;
         int t = 0;                                           // key tiles loaded so far
         int next = blockIdx.x;                               // the first of a CTA by its number, the others from the counter
@@ -798,15 +820,14 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
             }
             return true;
         };
-        for (int w = 0;; ++w) {
+        bool ok = lane == 0;
+        for (int w = 0; ok; ++w) {
             x.nt_a = -1;
             while (next < items && x.nt_a < 0) {             // to a slot that has rows
                 const int item = next;
-                unsigned taken = 0u;
-                if (lane == 0) taken = atomicAdd(a.counter, 1u);
+                next = (int)(gridDim.x + atomicAdd(a.counter, 1u));
                 x.hk = item % a.kv_heads;
-                const Seq s = find_sequence(a.cu, a.B, a.T, a.max_len, slots - 1 - item / a.kv_heads, two);
-                next = (int)(gridDim.x + __shfl_sync(0xffffffffu, taken, 0));
+                const Seq s = find_sequence_alone(a.cu, a.B, a.T, a.max_len, slots - 1 - item / a.kv_heads, two);
                 x.start = s.start, x.len = s.len, x.tok0 = s.local * two;
                 if (s.local < 0 || x.tok0 >= s.len) continue;
                 x.kv_slot = s.start / KT + (s.first_slot - s.start / two);
@@ -815,17 +836,14 @@ varlen_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constan
                 };
                 x.nt_a = tiles(x.tok0), x.nt_b = tiles(x.tok0 + a.tokens);
             }
-            int ok = 1;
-            if (lane == 0) {
-                ok = load(w) ? 1 : 0;
-                if (!ok) {                                   // copies in flight land before the block lets go of its memory
-                    note_timeout(a.status);
-                    for (int i = 0; i < kRing; ++i)
-                        for (uint32_t ph = 0; ph < 2; ++ph)
-                            mbar_wait_bounded(bar(W_KFULL + i), ph, 64u), mbar_wait_bounded(bar(W_VFULL + i), ph, 64u);
-                }
+            ok = load(w);
+            if (!ok) {                                       // copies in flight land before the block lets go of its memory
+                note_timeout(a.status);
+                for (int i = 0; i < kRing; ++i)
+                    for (uint32_t ph = 0; ph < 2; ++ph)
+                        mbar_wait_bounded(bar(W_KFULL + i), ph, 64u), mbar_wait_bounded(bar(W_VFULL + i), ph, 64u);
             }
-            if (!__shfl_sync(0xffffffffu, ok, 0) || x.nt_a < 0) break;
+            if (x.nt_a < 0) break;
         }
     } else if (warp == 9) {
         // ================= MMA issuer =================
