@@ -449,7 +449,10 @@ int i8tk_qk_norm_rope_quantize(const void* qkv, int dtype, int64_t row_stride, c
  *   out fp16 [tokens, heads, head_dim]; rows of no sequence (and behind a cut) are zero.
  * score[i][j] = (q_i.k_j) * sQ_i * sK_j / sqrt(D) for the j of i's sequence (j <= i when causal); what the
  * other positions hold, NaN and infinities included, does not reach the row.  A value scale that is
- * not finite makes the rows that see it NaN.
+ * not finite makes the rows that see it NaN.  Scores may have any size up to 2^126 log2 units (beyond
+ * it a row may be NaN).  The probability of a key times its value scale is one fp16 number: off by
+ * 2^-11 of itself, or by 2^-31 of the largest |v| of the sequence (of the positions that the row and
+ * its neighbours in the tile see) where that is more.
  * head_dim 64, 128 or 256; heads a multiple of kv_heads, at most 64 times as many; strides of Q, K,
  * V multiples of 16; Q, K, V and out 16-byte aligned; workspace
  * i8tk_attention_varlen_workspace_bytes(...) bytes, 256-byte aligned. */
@@ -492,6 +495,8 @@ int i8tk_kv4_dequantize(const void* pool, const int64_t* slots, void* k_f16, voi
  *        [0, num_pages) is not followed and recorded in the status block, a request of length 0
  *        gets zeros
  *   out  fp16 [batch, heads, head_dim]
+ * The probability of a position times its value scale is one fp16 number (2^-11 of itself, or a range of
+ * about 2^-36 of the largest such product).  Scores may have any size up to 2^126 log2 units.
  * heads a multiple of kv_heads, at most 16 times as many; head_dim 64 or 128; page_size 16, 32, 64
  * or 128; q_stride a multiple of 16; Q, pool and out 16-byte aligned; workspace 256-byte aligned. */
 size_t i8tk_decode_kv4_workspace_bytes(int batch, int heads, int kv_heads, int max_seq_len, int head_dim);

@@ -36,7 +36,8 @@
 // A row that one CTA scans whole is written there; a row cut between CTAs leaves at most two partial rows per CTA,
 // merged by a second kernel that is launched behind the first one's tail.
 // Measured: 32 requests up to 32768 positions, 32/8 heads, D 128, 64-position pages, 122-130 us a call (floor at the copy
-// rate: 95.8); 24 up to 4096, 12/12 heads, D 64: 19.7 us (6.8).  What bounds it is issue: 52 % of the slots, ALU pipe 54 %.
+// rate: 95.8); 24 up to 4096, 12/12 heads, D 64: 20 us (6.8).  No unit is full: 52 % of the issue slots at 16 warps an SM,
+// the ALU pipe, which unpacks, 54 %, memory 64 %; the empty slots are latency (fixed-latency dependencies, shared memory).
 #include "kv4.cuh"
 #include "score_reference.cuh"
 

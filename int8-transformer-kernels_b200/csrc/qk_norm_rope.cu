@@ -17,7 +17,7 @@
 // * r never touches the channels in the quantised form: it goes into the scale.
 // * Rounding is the addition of 1.5 * 2^23, the code is the low byte of the sum.
 // A row is held by D/8 lanes, eight channels (one 16-byte load) each; a warp has kRows rows per lane group in flight.
-// Measured: 8192 bf16 tokens, 32/8 heads, D 128, quantised: 44-45 us for 156 MB, 71 % of the issue slots (84 us before the
+// Measured: 8192 bf16 tokens, 32/8 heads, D 128, quantised: 42-44 us for 156 MB, 69 % of the issue slots (84 us before the
 // norm, weight and rotation were joined and the kinds of rotation split).
 #include "pairs16.cuh"
 

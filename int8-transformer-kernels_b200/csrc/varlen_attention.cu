@@ -5,14 +5,14 @@
 //
 // The tensor-core shape of prefill_attention.cu (Q.K^T as kind::i8 into tensor memory, P.V as kind::f16 with P read
 // from tensor memory, lazy maximum), with the differences below.  head_dim 256 runs it as it is (six sequences up to 1111,
-// 14/2 heads, not causal: 65 us); head_dim 64 and 128 run varlen_wide_kernel, which has its own comment:
+// 14/2 heads, not causal: 64-66 us); head_dim 64 and 128 run varlen_wide_kernel, which has its own comment:
 //
 // * A CTA's 128 query rows are floor(128/group) tokens of ALL the query heads that share a key head (row = token *
 //   group + head).  K and V tiles are then read once for the group, and with a causal mask the part of the last tiles
 //   that is computed and thrown away covers 128/group tokens instead of 128.  One three-dimensional TMA box brings
 //   the query tile from the caller's [token][head][channel] layout; rows past the box are never stored.
 // * Sequences are found on the device.  Sequence b owns the tile slots cu[b]/n + b .. cu[b+1]/n + b + 1 of n tokens
-//   each -- at least as many as it needs, for any lengths -- so a CTA finds its work by bisection and no plan runs
+//   each -- at least as many as it needs, for any lengths -- so a CTA finds its work by a search and no plan runs
 //   ahead; at most one slot per sequence and head is empty.
 // * P carries the values' scales: P_ij = fp16(p_ij * sV_j * c), and V enters as its codes, exact in fp16.  c is the
 //   power of two that brings the largest scale of the sequence and head to [2^6, 2^7), so P stays in range for any
@@ -617,7 +617,7 @@ varlen_attention_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 // comes from its first 32 scores.
 // The pairs of tiles are taken from a counter, long rows first, by the thread that starts the loads, which runs ahead
 // into the next pair while the last one is finished.
-// (8192 tokens causal, 32/8 heads, D 128: 540 us, 1.02 PFLOP/s; with prefill_attention.cu's shape 622.  Two score blocks of
+// (8192 tokens causal, 32/8 heads, D 128: 519-547 us, 1.02 PFLOP/s at 540; with prefill_attention.cu's shape 622.  Two score blocks of
 // 64 positions per query tile, Q.K^T a tile ahead: 592; halves of 64 with an issuing thread for each query tile: 585.)
 constexpr int kWideThreads = 12 * 32;    // 2 x 4 softmax warps, loads, MMA, and two that fill their warpgroup
 // Registers per thread: 168 at launch; the warpgroup of loads and MMA hands most of its own to the softmax warpgroups
